@@ -13,7 +13,7 @@ import threading
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("BRICKREC_LIB", os.path.join(HERE, "libbrickrec.so"))
 
-BB_F32, BB_BF16, BB_F64 = 0, 1, 2
+BB_F32, BB_BF16, BB_F64, BB_F16 = 0, 1, 2, 3
 BB_HOST, BB_DEVICE = 0, 1
 BB_MODE_SEMANTIC, BB_MODE_SIMILAR, BB_MODE_CF, BB_MODE_HYBRID = 0, 1, 2, 3
 BB_Q_OUT_KEYS = 1
@@ -27,7 +27,8 @@ BB_OK, BB_E_ARG, BB_E_HIP, BB_E_STATE, BB_E_NOMEM, BB_E_HOSTSYNC = 0, -1, -2, -3
 EXPORTS = ("bb_create", "bb_upload_items", "bb_upload_cf", "bb_upload_attrs", "bb_eval_mask",
            "bb_search", "bb_key_lens", "bb_finalize", "bb_set_profiling", "bb_get_profile", "bb_set_option",
            "bb_info", "bb_get_rows", "bb_create_view", "bb_destroy", "bb_last_error", "bb_abi_version",
-           "bb_plan_create", "bb_plan_launch", "bb_plan_destroy", "bb_check_dual_scan_args")
+           "bb_plan_create", "bb_plan_launch", "bb_plan_destroy", "bb_check_dual_scan_args",
+           "bb_quantize_fp8", "bb_scores_fp8", "bb_adjust_scores")
 
 
 class BrickrecError(RuntimeError):
@@ -67,6 +68,21 @@ class bb_profile(C.Structure):
                 ("names", C.c_char_p * 8), ("n", C.c_int32)]
 
 
+class bb_fp8_rows(C.Structure):
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("d", C.c_int64),
+                ("ld", C.c_int64), ("scales_ld", C.c_int64), ("tile", C.c_int32)]
+
+
+class bb_adjust(C.Structure):
+    _fields_ = [("scores", C.c_void_p), ("out", C.c_void_p), ("B", C.c_int64), ("n", C.c_int64),
+                ("ld_scores", C.c_int64), ("ld_out", C.c_int64), ("dtype", C.c_int32), ("ids64", C.c_int32),
+                ("seen", C.c_void_p), ("n_seen", C.c_int64), ("ld_seen", C.c_int64), ("seen_len", C.c_void_p),
+                ("repetition", C.c_void_p), ("presence", C.c_void_p), ("frequency", C.c_void_p),
+                ("repetition_all", C.c_float), ("presence_all", C.c_float), ("frequency_all", C.c_float),
+                ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("n_bias", C.c_int64), ("ld_bias", C.c_int64),
+                ("mask", C.c_void_p), ("ld_mask", C.c_int64)]
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -104,6 +120,10 @@ def load() -> C.CDLL:
             "bb_plan_launch": ([P], C.c_int),
             "bb_plan_destroy": ([P], C.c_int),
             "bb_check_dual_scan_args": ([C.c_int64], C.c_int),
+            "bb_quantize_fp8": ([C.c_int32, P, C.c_int32, C.c_int64, C.POINTER(bb_fp8_rows), P], C.c_int),
+            "bb_scores_fp8": ([C.c_int32, C.POINTER(bb_fp8_rows), C.POINTER(bb_fp8_rows), P, C.c_int32, C.c_int64, P],
+                              C.c_int),
+            "bb_adjust_scores": ([C.c_int32, C.POINTER(bb_adjust), P], C.c_int),
             "bb_last_error": ([], C.c_char_p),
             "bb_abi_version": ([], C.c_int),
         }

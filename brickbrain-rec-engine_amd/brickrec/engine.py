@@ -195,6 +195,7 @@ class ItemIndex:
                                                int(prenormalized), L.BB_HOST, bp)
             L.check(rc, "bb_upload_items")
             self.n_items, self.d = int(n), int(d)
+            self._fp8 = None
 
     def upload_cf(self, item_factors: np.ndarray, present: Optional[np.ndarray] = None):
         """CF item factors (n×r, same row space as the items) + presence mask (bool n)."""
@@ -522,6 +523,63 @@ class ItemIndex:
         if self.dtype != "f32":
             out = (out.astype(np.uint32) << 16).view(np.float32)
         return out
+
+    # ------------------------------------------------------------------ dense scores
+    def quantize_items(self, chunk: int = 65536):
+        """An 8-bit copy of the stored (normalised) rows, kept with this index and its views until the
+        next upload: 1 byte an element and 4 for each 128 of a row.  Returns it (``fp8.Fp8Rows``).
+        Synchronous, as an upload is."""
+        import torch
+        from .fp8 import Fp8Rows, quantize_rows
+        root = getattr(self, "_base", None) or self
+        if self.n_items <= 0:
+            raise L.BrickrecError("no items uploaded")
+        dev = torch.device("cuda", self.device)
+        with torch.cuda.device(dev):
+            rows = Fp8Rows.empty(self.n_items, self.d, device=dev)
+            for a in range(0, self.n_items, chunk):
+                b = min(self.n_items, a + chunk)
+                ids = torch.arange(self.id_offset + a, self.id_offset + b, device=dev)
+                quantize_rows(self.get_rows(ids), out=rows.part(a, b))
+            torch.cuda.current_stream(dev).synchronize()
+        root._fp8 = rows
+        return rows
+
+    def scores(self, q_rows, *, normalize: bool = True, dtype=None, stream=None, out=None, **adjust):
+        """Dense scores [B, n] of query rows against the 8-bit copy of the items (``quantize_items``,
+        called first): column j is item id_offset + j.  The queries are L2-normalised unless
+        ``normalize`` is False (a zero row scores 0), then quantised as the items are; the scores
+        are those of the 8-bit rows, not the exact ones that ``search`` ranks by.  ``adjust``: the
+        penalties, biases and mask of ``adjust.adjust_scores``, applied in place.  Every stored row gets
+        a score; pass a mask to leave rows out.
+
+        Numpy in -> numpy out (f32); torch CUDA rows -> a torch tensor of ``dtype`` (f32 by default),
+        asynchronously on ``stream`` (default: torch's current stream)."""
+        import torch
+        from .adjust import adjust_scores
+        from .fp8 import quantize_rows, scores_fp8
+        root = getattr(self, "_base", None) or self
+        items = getattr(root, "_fp8", None)
+        if items is None:
+            raise L.BrickrecError("scores() needs quantize_items() first")
+        dev = torch.device("cuda", self.device)
+        host = not _is_torch(q_rows)
+        if host:
+            q_rows = torch.from_numpy(np.ascontiguousarray(q_rows, dtype=np.float32)).to(dev)
+        if q_rows.dim() != 2 or q_rows.shape[1] != self.d:
+            raise ValueError(f"query rows are [B, {self.d}]: got {tuple(q_rows.shape)}")
+        s = stream if stream is not None else torch.cuda.current_stream(dev)
+        used = [q_rows, items.codes, items.scales] + [t for t in (out, *adjust.values()) if t is not None and _is_torch(t)]
+        for t in used:  # (their memory stays theirs until the stream has passed this call)
+            t.record_stream(s)
+        with torch.cuda.stream(s):
+            q = q_rows.float() if normalize or q_rows.dtype == torch.float64 else q_rows
+            if normalize:
+                q = torch.nn.functional.normalize(q, dim=1, eps=1e-30)
+            r = scores_fp8(quantize_rows(q), items, dtype=dtype or torch.float32, out=out)
+            if adjust:
+                adjust_scores(r, out=r, **adjust)
+        return r.cpu().numpy() if host else r
 
     # ------------------------------------------------------------------ options
     def set_option(self, option: str, value: int):

@@ -123,6 +123,14 @@ class SemanticIndex:
             q = q[None, :]
         return self.index.search("semantic", k, q_rows=q, mask=mask)
 
+    def scores(self, queries, **kw):
+        """Dense scores [B, n] of query vectors against an 8-bit copy of the embeddings, with penalties,
+        biases and masks (``ItemIndex.scores``; the copy is made at the first call)."""
+        if getattr(self.index, "_fp8", None) is None:
+            self.index.quantize_items()
+        q = np.asarray(queries, np.float32) if isinstance(queries, (list, tuple)) else queries
+        return self.index.scores(q[None, :] if q.ndim == 1 else q, **kw)
+
     def similar_to(self, set_nums: Sequence[str], k: int, mask: Optional[np.ndarray] = None):
         """Similar sets of stored rows (rank 0 = the arg-max dropped, as get_similar_sets)."""
         rows = np.array([self.pos[s] for s in set_nums], np.int64)

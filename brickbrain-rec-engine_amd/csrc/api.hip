@@ -17,6 +17,7 @@
 #include <vector>
 
 #include "../../include/brickrec.h"
+#include "abi.h"
 #include "common.h"
 #include "list_epi.h"
 #include "sq.h"
@@ -105,6 +106,8 @@ bool live_has_magic(const H* p, uint64_t magic) {
 }
 
 }  // namespace
+
+int bb::abi_fail(int code, const std::string& msg) { return fail(code, msg); }
 
 struct bb_index {
   uint64_t magic = kIndexMagic;

@@ -44,6 +44,7 @@ extern "C" {
 #define BB_F32 0
 #define BB_BF16 1
 #define BB_F64 2           /* host input only: converted (after f64 normalisation) */
+#define BB_F16 3           /* the 8-bit rows' inputs and scores only (bb_quantize_fp8 and after) */
 
 /* pointer location */
 #define BB_HOST 0
@@ -276,6 +277,70 @@ int bb_plan_destroy(bb_plan* plan);
  * stride `ldx`, else BB_E_ARG naming the broken rule — the scan's LDS-DMA source offsets are 24-bit,
  * so a stride >= 2^23 is refused before any launch instead of faulting. */
 int bb_check_dual_scan_args(int64_t ldx);
+
+/* ---- 8-bit rows and dense scores (no reference counterpart) ---------------------------------
+ * These calls need no index: every pointer is a device pointer on `device` (-1 = the current
+ * device), and the work goes out on `stream` (a hipStream_t; NULL = the null stream) without a
+ * synchronisation, an allocation, a fill or a copy, so a call can be captured into a graph.  They
+ * keep no state between calls and may run from several threads. */
+
+/* Rows of 8-bit floating point (e4m3: 448 the largest, no infinities) with an f32 scale for
+ * each block: element (i, j) is codes[i*ld + j] * scales[(j/128)*scales_ld + i], or with
+ * tile != 0 * scales[(j/128)*scales_ld + i/128] (blocks of 128 x 128).  Each row holds
+ * ceil(d/128)*128 codes, those from d on zero.  codes: 16-byte aligned, ld a multiple of 16 and
+ * at least that; scales: 4-byte aligned, scales_ld at least the scales of one block column. */
+typedef struct {
+  uint8_t* codes;
+  float* scales;
+  int64_t rows, d;
+  int64_t ld, scales_ld;
+  int32_t tile;
+} bb_fp8_rows;
+
+/* Rows x (out->rows x out->d, dtype BB_F32 / BB_BF16 / BB_F16, ldx elements between rows) into
+ * 8-bit rows.  A block whose largest magnitude is a (at least 2^-100) has scale a/448 and codes
+ * x*(448/a) rounded to the nearest, ties to even, all in f32.  A block that holds an infinity
+ * or a NaN has scale NaN and codes 0, so that every score that reads it is NaN. */
+int bb_quantize_fp8(int32_t device, const void* x, int32_t dtype, int64_t ldx, const bb_fp8_rows* out, void* stream);
+
+/* out[m][n] = <q row m, item row n> for every pair, ldo elements between rows of out, dtype BB_F32 /
+ * BB_BF16 / BB_F16 (rounded once, to nearest even).  q->d == items->d; q->tile must be 0.
+ * Products of codes are exact and summed in f32 over each block of 128, then multiplied by the two
+ * scales (their product first) and summed over the blocks in f32, in ascending order up to a split
+ * into a few parts; the order depends on the sizes alone, so equal calls give equal bits. */
+int bb_scores_fp8(int32_t device, const bb_fp8_rows* q, const bb_fp8_rows* items, void* out, int32_t dtype,
+                  int64_t ldo, void* stream);
+
+/* Penalties, biases and a mask on B x n scores (or logits), in f32 and rounded once:
+ *   c = how often id v stands in the row's seen list
+ *   c > 0:  s = (s > 0 ? s / repetition : s * repetition) - (frequency * c + presence)
+ *   s += the bias of v, if the row's bias list holds v (the last entry where it does so twice)
+ *   s = -infinity where the mask's bit v is 0, whatever s was (NaN too)
+ * Ids outside [0, n) are skipped (lists padded with -1). */
+typedef struct {
+  const void* scores;        /* B x n of `dtype`, ld_scores elements between rows            */
+  void* out;                 /* the same shape and type, ld_out between rows; may be scores
+                                itself with the same ld; may not overlap it otherwise        */
+  int64_t B, n;
+  int64_t ld_scores, ld_out;
+  int32_t dtype;             /* BB_F32 / BB_BF16 / BB_F16                                    */
+  int32_t ids64;             /* bit 0: seen is int64, bit 1: bias_ids is int64 (int32 if not)*/
+  const void* seen;          /* B x n_seen ids, ld_seen between rows (0: one list for all);
+                                NULL = none                                                  */
+  int64_t n_seen, ld_seen;
+  const int32_t* seen_len;   /* [B] entries of each row that count; NULL = all n_seen; values
+                                outside [0, n_seen] count as the nearer end                  */
+  const float *repetition, *presence, *frequency;  /* [B] each; NULL = the value for all rows */
+  float repetition_all, presence_all, frequency_all;
+  const void* bias_ids;      /* B x n_bias ids and their biases, ld_bias between the rows of
+                                both (0: one list for all); NULL = none                      */
+  const float* bias;
+  int64_t n_bias, ld_bias;
+  const uint32_t* mask;      /* ceil(n/32) words a row, ld_mask words between rows (0: one
+                                mask for all, as bb_eval_mask writes it); NULL = none        */
+  int64_t ld_mask;
+} bb_adjust;
+int bb_adjust_scores(int32_t device, const bb_adjust* a, void* stream);
 
 int bb_info(bb_index* idx, int64_t* n_items, int32_t* d, int32_t* d_pad, int32_t* r);
 /* Handles are checked by every entry point: a destroyed, foreign or corrupted bb_index /

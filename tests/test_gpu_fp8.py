@@ -1,0 +1,307 @@
+"""8-bit rows on the device: codes and scales bit for bit as the f32 rule gives them, scores within a
+derived bound of the f64 product (tests/_fp8_ref.py), the layouts, streams and captures that the calls
+allow, and the index's own dense scores."""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import _fp8_ref as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def br():
+    if not torch.cuda.is_available():
+        pytest.fail("GPU tests need a ROCm device")
+    import brickrec
+    return brickrec
+
+
+def make(n, d, dtype=torch.float32, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((n, d), generator=g) * torch.exp(torch.randn((n, 1), generator=g))
+    return x.to(dtype)
+
+
+def quantized(br, n, d, tile=False, seed=0):
+    return br.quantize_rows(make(n, d, seed=seed).to(DEV), tile=tile)
+
+
+def check_scores(q, x, got):
+    y, tol = R.scores_bound(R.values(q.codes.cpu(), q.scales.cpu(), q.tile), R.values(x.codes.cpu(), x.scales.cpu(), x.tile),
+                            got.dtype)
+    off = (got.double().cpu() - y).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
+
+
+# ---- quantising -----------------------------------------------------------------------------
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n, d", [(1, 1), (1, 128), (3, 127), (33, 129), (128, 384), (129, 50), (200, 1000), (257, 4097)])
+def test_quantize(br, n, d, dtype, tile):
+    x = make(n, d, dtype, seed=n + d)
+    codes, scales = R.quantize(x, tile)
+    got = br.quantize_rows(x.to(DEV), tile=tile)
+    assert torch.equal(got.codes.cpu().float(), codes.float())
+    assert torch.equal(got.scales.cpu(), scales)
+    # the values are within half a step: 2^-4 of the value, or half of 2^-9 of the scale below 2^-6,
+    # with the f32 roundings of the scale, the inverse and the product
+    off = (got.dequantize().cpu().double() - x.double()).abs()
+    s = scales.double().t().repeat_interleave(128, 1)[:, :d]
+    s = s.repeat_interleave(128, 0)[:n] if tile else s
+    assert bool((off <= (x.double().abs() * 2.0 ** -4 + s * 2.0 ** -10) * (1 + 2.0 ** -20)).all())
+
+
+@pytest.mark.parametrize("tile", [False, True])
+def test_quantize_special_values(br, tile):
+    x = make(300, 400, seed=5)
+    x[0] = 0.0                      # a block of zeros
+    x[1] *= 1e-38                   # denormal after scaling, below the floor
+    x[2] = 3e38
+    x[130, 5] = float("inf")
+    x[131, 200] = float("nan")
+    x[290, 399] = -float("inf")
+    codes, scales = R.quantize(x, tile)
+    got = br.quantize_rows(x.to(DEV), tile=tile)
+    assert torch.equal(got.codes.cpu().float(), codes.float())
+    assert torch.equal(torch.nan_to_num(got.scales.cpu(), nan=-1.0), torch.nan_to_num(scales, nan=-1.0))
+    assert torch.isnan(scales).any()
+    # a score that reads such a block is NaN, every other one is not
+    q = br.quantize_rows(make(4, 400).to(DEV))
+    nan = torch.isnan(br.scores_fp8(q, got)).cpu()
+    bad = torch.isnan(scales).any(0)
+    bad = bad.repeat_interleave(128)[:300] if tile else bad
+    assert torch.equal(nan, bad[None, :].expand(4, 300))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_strided_and_misaligned(br, dtype):
+    big = make(40, 700, dtype, seed=9).to(DEV)
+    for x in (big[:, 3:390], big[::2, 1:], big.t()[5:300], big[:1].expand(7, 700), big[7:8, 5:6]):
+        codes, scales = R.quantize(x.cpu())
+        got = br.quantize_rows(x)
+        assert torch.equal(got.codes.cpu().float(), codes.float()) and torch.equal(got.scales.cpu(), scales)
+
+
+def test_quantize_into_parts(br):
+    x = make(500, 300, seed=3).to(DEV)
+    for tile in (False, True):
+        whole = br.quantize_rows(x, tile=tile)
+        out = br.Fp8Rows.empty(500, 300, tile, DEV)
+        for a, b in ((0, 128), (128, 384), (384, 500)):
+            br.quantize_rows(x[a:b], tile=tile, out=out.part(a, b))
+        assert torch.equal(out.codes.view(torch.uint8), whole.codes.view(torch.uint8))
+        assert torch.equal(out.scales, whole.scales)
+
+
+# ---- the product ----------------------------------------------------------------------------
+SIZES = [(1, 1, 1), (1, 64, 128), (1, 25216, 384), (2, 65, 129), (15, 257, 640), (16, 1000, 2048), (17, 127, 4096),
+         (33, 513, 384), (64, 300, 256), (65, 4100, 128), (100, 129, 1000), (128, 128, 4224), (129, 255, 96), (250, 777, 777),
+         (256, 256, 512), (257, 1025, 384), (512, 2050, 1280), (700, 515, 2100)]
+
+
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k", SIZES)
+def test_scores(br, m, n, k, dtype, tile):
+    q, x = quantized(br, m, k, seed=1), quantized(br, n, k, tile, seed=2)
+    check_scores(q, x, br.scores_fp8(q, x, dtype=dtype))
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 70, 128), (20, 130, 300), (300, 270, 256)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_into_strided_rows(br, m, n, k, dtype):
+    q, x = quantized(br, m, k, seed=1), quantized(br, n, k, seed=2)
+    want = br.scores_fp8(q, x, dtype=dtype)
+    buf = torch.full((m + 2, n + 9), 7.0, dtype=dtype, device=DEV)
+    out = buf[1:m + 1, 3:n + 3]
+    assert br.scores_fp8(q, x, out=out) is out
+    assert torch.equal(out, want)
+    buf[1:m + 1, 3:n + 3] = 7.0
+    assert bool((buf == 7.0).all())
+
+
+def test_scores_of_parts(br):
+    q, x = quantized(br, 50, 500, seed=1), quantized(br, 700, 500, seed=2)
+    whole = br.scores_fp8(q, x)
+    assert torch.equal(br.scores_fp8(q, x.part(100, 300)), whole[:, 100:300])
+    y = quantized(br, 700, 500, True, seed=2)
+    assert torch.equal(br.scores_fp8(q, y.part(128, 700)), br.scores_fp8(q, y)[:, 128:])
+
+
+def test_rows_further_apart_than_32_bits(br):
+    # codes and scores whose offsets pass 2^32: three rows, 2^31 + 4096 bytes apart
+    ld = (1 << 31) + 4096
+    store = torch.empty(2 * ld + 1024, dtype=torch.uint8, device=DEV)
+    far = torch.as_strided(store, (3, 256), (ld, 1)).view(torch.float8_e4m3fn)
+    near = quantized(br, 3, 200, seed=4)
+    out = br.Fp8Rows(far, torch.empty_like(near.scales), 200)
+    br.quantize_rows(make(3, 200, seed=4).to(DEV), out=out)
+    assert torch.equal(far.float(), near.codes.float())
+    q = quantized(br, 5, 200, seed=5)
+    assert torch.equal(br.scores_fp8(q, out), br.scores_fp8(q, near))
+    assert torch.equal(br.scores_fp8(out, q), br.scores_fp8(near, q))
+    del far, out, store
+    buf = torch.empty(2 * ld + 1024, dtype=torch.float16, device=DEV)
+    y = torch.as_strided(buf, (3, 5), (ld, 1))
+    br.scores_fp8(near, q, out=y)
+    assert torch.equal(y, br.scores_fp8(near, q, dtype=torch.float16))
+
+
+def test_scores_span_many_items(br):
+    # more than 2^32 bytes of scores, checked at both ends against the parts
+    q, x = quantized(br, 600, 128, seed=1), quantized(br, 2000, 128, seed=2)
+    reps = 1000
+    big = br.Fp8Rows(x.codes.view(torch.uint8).repeat(reps, 1).view(torch.float8_e4m3fn), x.scales.repeat(1, reps), 128)
+    y = br.scores_fp8(q, big, dtype=torch.float32)
+    want = br.scores_fp8(q, x)
+    assert torch.equal(y[:, :2000], want) and torch.equal(y[:, -2000:], want) and torch.equal(y[:, 10 ** 6:10 ** 6 + 2000], want)
+
+
+@pytest.mark.parametrize("m, n, k, dtype", [(8, 4096, 1024, torch.bfloat16), (300, 600, 512, torch.float32)])
+def test_scores_replayed(br, m, n, k, dtype):
+    q, x = quantized(br, m, k, seed=1), quantized(br, n, k, seed=2)
+    raw = make(m, k, seed=1).to(DEV)
+    out = torch.zeros((m, n), dtype=dtype, device=DEV)
+    br.scores_fp8(q, x, out=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        br.scores_fp8(br.quantize_rows(raw, out=q), x, out=out)
+    for s in range(4):
+        raw.copy_(make(m, k, seed=10 + s))
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        want = br.scores_fp8(br.quantize_rows(raw), x, dtype=dtype)
+        assert torch.equal(out, want), s
+        want.sum().item()
+
+
+def test_scores_on_streams_and_threads(br):
+    x = quantized(br, 5000, 384, seed=2)
+    qs = [quantized(br, 40, 384, seed=20 + i) for i in range(4)]
+    want = [br.scores_fp8(q, x) for q in qs]
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        s = torch.cuda.Stream(DEV)
+        for _ in range(10):
+            got[i] = br.scores_fp8(qs[i], x, stream=s)
+        s.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_refusals(br):
+    q, x = quantized(br, 3, 200), quantized(br, 5, 200, True)
+    with pytest.raises(br.BrickrecError):
+        br.scores_fp8(x, q)                              # tiles as queries
+    with pytest.raises(br.BrickrecError):
+        br.scores_fp8(q, quantized(br, 5, 201))
+    with pytest.raises(TypeError):
+        br.scores_fp8(q, x, dtype=torch.float64)
+    with pytest.raises(ValueError):
+        br.scores_fp8(q, x, out=torch.empty((3, 6), device=DEV))
+    with pytest.raises(ValueError):
+        br.scores_fp8(q, x, out=torch.empty((5, 3), device=DEV).t())
+    with pytest.raises(TypeError):
+        br.scores_fp8(q, x, out=torch.empty((3, 5), dtype=torch.int32, device=DEV))
+    with pytest.raises(ValueError):
+        br.Fp8Rows(q.codes, q.scales, 300)
+    with pytest.raises(ValueError):
+        br.Fp8Rows(q.codes, q.scales[:, :2], 200)
+    with pytest.raises(TypeError):
+        br.Fp8Rows(q.codes.view(torch.uint8), q.scales, 200)
+    with pytest.raises(TypeError):
+        br.quantize_rows(torch.zeros((3, 5), dtype=torch.float64, device=DEV))
+    with pytest.raises(ValueError):
+        br.quantize_rows(torch.zeros(5, device=DEV))
+    with pytest.raises(ValueError):
+        br.quantize_rows(torch.zeros((3, 200), device=DEV, requires_grad=True))
+    with pytest.raises(ValueError):
+        br.quantize_rows(torch.zeros((3, 200), device=DEV), out=x)
+    with pytest.raises(ValueError):
+        x.part(1, 3)
+    assert br.scores_fp8(quantized(br, 0, 200), x).shape == (0, 5)
+    assert br.quantize_rows(torch.zeros((4, 0), device=DEV)).codes.shape == (4, 0)
+
+
+# ---- a run of them together -------------------------------------------------------------------
+def test_weights_activations_scores_adjusted(br):
+    """Quantised activations against quantised weights, the logits adjusted in place: against f64 from the
+    unquantised inputs, by e4m3's half step 2^-4 on each factor (and 2^-10 of the block's scale)."""
+    m, n, k = 12, 1500, 640
+    a, w = make(m, k, torch.bfloat16, seed=1), make(n, k, torch.bfloat16, seed=2)
+    qa, qw = br.quantize_rows(a.to(DEV)), br.quantize_rows(w.to(DEV), tile=True)
+    logits = br.scores_fp8(qa, qw, dtype=torch.float32)
+    g = torch.Generator().manual_seed(3)
+    seen = torch.randint(-1, n, (m, 40), generator=g, dtype=torch.int32)
+    allowed = torch.rand((m, n), generator=g) < 0.7
+    y = br.adjust_scores(logits, seen=seen.to(DEV), repetition=1.3, presence=0.2, frequency=0.1, mask=allowed.to(DEV),
+                         out=logits).cpu().double()
+    va, vw = a.double(), w.double()
+    ea, ew = (R.values(q.codes.cpu(), q.scales.cpu(), q.tile)[:, :k] - v for q, v in ((qa, va), (qw, vw)))
+    plain, _ = R.adjust((va @ vw.t()).float(), seen, None, 1.3, 0.2, 0.1, mask=allowed)
+    tol = 1.3 * (va.abs() @ ew.abs().t() + ea.abs() @ (vw.abs() + ew.abs()).t()) + 1e-3 * (va.abs() @ vw.abs().t())
+    assert torch.equal(torch.isinf(y), ~allowed)
+    assert bool(((y - plain).abs()[allowed] <= tol[allowed]).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_index_scores(br, dtype):
+    n, d, B = 3001, 384, 9
+    x, q = make(n, d, seed=1), make(B, d, seed=2)
+    idx = br.ItemIndex(device=0, dtype=dtype, id_offset=100)
+    with pytest.raises(br.BrickrecError):
+        idx.quantize_items()
+    idx.upload_items(x.numpy())
+    with pytest.raises(br.BrickrecError):
+        idx.scores(q.to(DEV))
+    rows = idx.quantize_items(chunk=1000)
+    stored = torch.from_numpy(np.asarray(idx.get_rows(np.arange(100, 100 + n))))
+    codes, scales = R.quantize(stored)
+    assert torch.equal(rows.codes.cpu().float(), codes.float()) and torch.equal(rows.scales.cpu(), scales)
+    got = idx.scores(q.to(DEV))
+    assert torch.equal(torch.from_numpy(idx.scores(q.numpy())), got.cpu())
+    unit = torch.nn.functional.normalize(q.to(DEV), dim=1, eps=1e-30)
+    assert torch.equal(got, br.scores_fp8(br.quantize_rows(unit), rows))
+    # within e4m3's half steps of the exact cosine: 2^-4 of each factor, and their product
+    cos = torch.nn.functional.normalize(q.double(), dim=1) @ torch.nn.functional.normalize(x.double(), dim=1).t()
+    assert float((got.cpu().double() - cos).abs().max()) < 2 * 2.0 ** -4 + 2.0 ** -7
+    idx.upload_attrs(np.arange(n), np.full(n, 2015), np.zeros(n, np.int32))
+    bits = idx.eval_mask_bits(br.Predicate(parts_min=100, parts_max=2000))
+    view = idx.view()
+    s = torch.cuda.Stream(DEV)
+    seen = torch.tensor([[5, 7, 7, -1]] * B, dtype=torch.int32, device=DEV)
+    torch.cuda.synchronize()
+    y = view.scores(q.to(DEV), stream=s, mask=bits, seen=seen, frequency=0.5, presence=0.25)
+    s.synchronize()
+    want = got.clone()
+    want[:, 5] -= 0.75
+    want[:, 7] -= 1.25
+    want[:, :100] = -float("inf")
+    want[:, 2001:] = -float("inf")
+    assert torch.equal(y, want)
+    view.close()
+    idx.upload_items(x.numpy())
+    with pytest.raises(br.BrickrecError):
+        idx.scores(q.to(DEV))
+    idx.close()
+
+
+def test_semantic_scores(br):
+    from brickrec.semantic import SemanticIndex
+    x = make(500, 64, seed=1)
+    sem = SemanticIndex([f"s{i}" for i in range(500)], x.numpy())
+    one = sem.scores(x[7].numpy())
+    assert one.shape == (1, 500) and int(one[0].argmax()) == 7
+    assert np.array_equal(sem.scores([x[7].tolist(), x[8].tolist()])[:1], one)
