@@ -210,58 +210,376 @@ __device__ __forceinline__ typename M::Frag load32(const uint8_t* p) {
   return M::make(*(const u32x4*)p, *(const u32x4*)(p + 16));
 }
 
-// 16 consecutive scores of one row from column n, as many as are inside.
-template <typename T>
-__device__ __forceinline__ void store16(T* row, int64_t n, int64_t N, const f32x4 (&acc)[4]) {
-  typedef typename Vec8<T>::type V;
-  if (n + 16 <= N) {
+// ---- the product of few rows -----------------------------------------------------------------
+// Bound by reading the items once: operands go straight from memory to registers, up to PF blocks
+// of a wave in flight.  A wave holds 16 NT items x 16 MT queries; the KS waves of a workgroup take every
+// KS-th block of the same rows and are summed through LDS, in order of the wave.
+template <typename T, int NT, int MT, int KS, int PF>
+__global__ __launch_bounds__(KS * 64) void product_few_kernel(ProductArgs a, int n_groups) {
+  typedef typename Mode<T>::Frag Frag;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)(blockIdx.x % n_groups) * 16 * NT, m0 = (int64_t)(blockIdx.x / n_groups) * 16 * MT;
+  const uint8_t *xp[NT], *qp[MT];
+  const float *xs[NT], *qs[MT];
+  const bool whole = n0 + 16 * NT <= a.N;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      V v;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (T)acc[2 * h + (j >> 2)][j & 3];
-      *(V*)(row + n + 8 * h) = v;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (n + j < N) row[n + j] = (T)acc[j >> 2][j & 3];
-  }
-}
-
-// A wave holds 64 items x 16 queries; operands straight from memory.  Item row p of MFMA tile t
-// is item 16 (p >> 2) + 4 t + (p & 3) of the 64, so that a lane's 16 results are 16
-// consecutive items of its query.
-template <typename T>
-__global__ __launch_bounds__(256) void product_kernel(ProductArgs a, int n_groups) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t n0 = ((int64_t)(blockIdx.x % n_groups) * 4 + wave) * 64;
-  const int64_t m = (int64_t)(blockIdx.x / n_groups) * 16 + r;
-  if (n0 >= a.N) return;
-  const int64_t mc = m < a.M ? m : a.M - 1;
-  const uint8_t* qp = a.q + mc * a.ldq + g * 32;
-  const uint8_t* xp[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int64_t n = n0 + (r >> 2) * 16 + t * 4 + (r & 3);
+  for (int t = 0; t < NT; ++t) {
+    const int64_t n = n0 + t * 16 + r;
     xp[t] = a.x + (n < a.N ? n : a.N - 1) * a.ldx + g * 32;
+    const int64_t s = n0 + t * 16 + g * 4;
+    xs[t] = a.xs + (a.tile ? n0 / kBlock : s < a.N ? s : a.N - 1);
   }
-  f32x4 acc[4] = {};
-  for (int b = 0; b < a.kb; ++b) {
-    const auto q = load32<Mode<T>>(qp + (int64_t)b * kBlock);
-    const float sq = a.qs[b * a.ldqs + mc];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const f32x4 p = Mode<T>::dot(load32<Mode<T>>(xp[t] + (int64_t)b * kBlock), q);
+  for (int t = 0; t < MT; ++t) {
+    const int64_t m = m0 + t * 16 + r < a.M ? m0 + t * 16 + r : a.M - 1;
+    qp[t] = a.q + m * a.ldq + g * 32;
+    qs[t] = a.qs + m;
+  }
+  f32x4 acc[MT][NT] = {};
+  for (int b0 = wave; b0 < a.kb; b0 += KS * PF) {
+    u32x4 x[PF][NT][2], q[PF][MT][2];
+    f32x4 sx[PF][NT];
+    float sq[PF][MT];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t n = n0 + g * 16 + t * 4 + j;
-        const float sx = a.xs[b * a.ldxs + (a.tile ? n0 / kBlock : n < a.N ? n : a.N - 1)];
-        acc[t][j] = fmaf(sq * sx, p[j], acc[t][j]);
+    for (int f = 0; f < PF; ++f) {
+      const int b = b0 + f * KS < a.kb ? b0 + f * KS : b0;  // (a block past the end counts 0 below)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const u32x4* p = (const u32x4*)(xp[t] + (int64_t)b * kBlock);
+        x[f][t][0] = p[0];
+        x[f][t][1] = p[1];
+      }
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const u32x4* p = (const u32x4*)(qp[t] + (int64_t)b * kBlock);
+        q[f][t][0] = p[0];
+        q[f][t][1] = p[1];
+        sq[f][t] = qs[t][b * a.ldqs];
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float* p = xs[t] + b * a.ldxs;
+        if (a.tile) {
+          sx[f][t] = f32x4{*p, *p, *p, *p};
+        } else if (whole) {
+          typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+          sx[f][t] = *(const f32x4u*)p;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sx[f][t][j] = n0 + t * 16 + g * 4 + j < a.N ? p[j] : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < PF; ++f) {
+      if (b0 + f * KS >= a.kb) break;
+      Frag xf[NT];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) xf[t] = Mode<T>::make(x[f][t][0], x[f][t][1]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const Frag qf = Mode<T>::make(q[f][mt][0], q[f][mt][1]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const f32x4 p = Mode<T>::dot(xf[t], qf);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[mt][t][j] = fmaf(sq[f][mt] * sx[f][t][j], p[j], acc[mt][t][j]);
+        }
       }
     }
   }
-  if (m < a.M) store16((T*)a.out + m * a.ldo, n0 + g * 16, a.N, acc);
+  if constexpr (KS > 1) {
+    __shared__ f32x4 part[KS - 1][MT * NT][64];
+    if (wave > 0) {
+#pragma unroll
+      for (int i = 0; i < MT * NT; ++i) part[wave - 1][i][lane] = acc[i / NT][i % NT];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < KS - 1; ++w)
+#pragma unroll
+      for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += part[w][i][lane];
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int64_t m = m0 + mt * 16 + r;
+    if (m >= a.M) continue;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      typedef T Out __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+      const int64_t n = n0 + t * 16 + g * 4;
+      T* p = (T*)a.out + m * a.ldo + n;
+      if (n + 4 <= a.N) {
+        *(Out*)p = Out{(T)acc[mt][t][0], (T)acc[mt][t][1], (T)acc[mt][t][2], (T)acc[mt][t][3]};
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < a.N) p[j] = (T)acc[mt][t][j];
+      }
+    }
+  }
+}
+
+// ---- the product of many rows: tiles staged through LDS ----------------------------------------
+// A workgroup of WN x WM waves computes 64 WN items x 16 MT WM queries; a wave 64 items x 16 MT
+// queries.  Both operands' blocks of 128 codes go to LDS by LDS-DMA, double buffered: the next
+// block's loads are in flight while this one's products run, one barrier to a block.  The block's
+// scales go along (4 bytes a row).
+//
+// LDS rows are 128 bytes of 8 chunks; chunk c of row r sits at position c ^ f(r), with f such that the 8
+// rows that 8 neighbouring lanes read together have 8 different f: their 16-byte reads then fall
+// on all banks once.  A lane takes chunks g and g + 4 of its row (g = lane >> 4).
+//
+// Item rows are dealt to MFMA tiles so that a lane's results of V neighbouring tiles are 4 V
+// consecutive items: 16-byte stores, 64 bytes of a score row to each 4 lanes.
+template <typename T, int WN, int WM, int MT, int D>
+struct TileShape {
+  static constexpr int kWaves = WN * WM, kThreads = kWaves * 64;
+  static constexpr int V = 4 / (int)sizeof(T);
+  static constexpr int TN = WN * 64, TM = WM * MT * 16;
+  static constexpr int kX = TN * kBlock, kQ = TM * kBlock, kS = (TN + TM) * 4;
+  static constexpr int kStage = kX + kQ + kS;
+  static constexpr int kXP = TN / 8 / kWaves, kQP = TM / 8 / kWaves;  // 1-KiB pieces of a wave
+  static_assert(TN % (8 * kWaves) == 0 && TM % (8 * kWaves) == 0, "whole pieces for every wave");
+  static constexpr int kSP = ((TN + TM) / 64 + kWaves - 1) / kWaves;   // 64-scale pieces of a wave
+  static constexpr int kLoads = kXP + kQP + kSP;                       // loads of a wave and stage
+  static_assert(TN % 64 == 0 && TM % 64 == 0, "whole pieces of 64 scales");
+  static constexpr int kOut = TN * TM * (int)sizeof(T);                // the tile's scores, at the end
+  static constexpr int kLds = D * kStage > kOut ? D * kStage : kOut;
+  static_assert(D >= 2 && kLds <= 160 * 1024, "the stages fit the LDS");
+  static_assert((D - 2) * kLoads < 64, "the wait counter holds the loads in flight");
+  static __device__ __forceinline__ int fx(int n) { return (n & 3) | ((n >> (V == 1 ? 2 : 3)) & 1) << 2; }
+};
+
+template <int BYTES>
+__device__ __forceinline__ void lds_dma(uint32_t dst, uint32_t off, const void* base) {
+  static_assert(BYTES == 4 || BYTES == 16, "dword and four-dword pieces");
+  // (inline, so that the compiler's own waits leave these loads in flight)
+  if constexpr (BYTES == 16)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+}
+template <typename P>
+__device__ __forceinline__ P* uniform(P* p) {
+  const uint64_t v = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
+  return (P*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Workgroup -> tile: each XCD takes one contiguous run of tiles (its L2 then holds their rows), in
+// which up to 8 query tiles pass over the item tiles together.
+__device__ __forceinline__ void tile_of(int L, int total, int tiles_m, int tiles_n, int& tm, int& tn) {
+  const int xcd = L & 7, q8 = total >> 3, r8 = total & 7;
+  const int i = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (L >> 3);
+  const int band = i / (8 * tiles_n), m0 = band * 8, rows = tiles_m - m0 < 8 ? tiles_m - m0 : 8;
+  const int j = i - band * 8 * tiles_n;
+  tm = m0 + j % rows;
+  tn = j / rows;
+}
+
+template <typename T, bool TILE, int WN, int WM, int MT, int D>
+__global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
+  using S = TileShape<T, WN, WM, MT, D>;
+  constexpr int V = S::V;
+  __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
+  int tm, tn;
+  tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+  const int64_t n0 = (int64_t)tn * S::TN, m0 = (int64_t)tm * S::TM;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wn = wave % WN, wm = wave / WN;
+  const int nx = (int)(a.N - n0 < S::TN ? a.N - n0 : S::TN), nq = (int)(a.M - m0 < S::TM ? a.M - m0 : S::TM);
+
+  // this lane's source offsets (rows past the end repeat the last one; the host keeps 256 rows under 2^32 bytes)
+  uint32_t xoff[S::kXP], qoff[S::kQP];
+#pragma unroll
+  for (int p = 0; p < S::kXP; ++p) {
+    const int row = (wave * S::kXP + p) * 8 + (lane >> 3);
+    xoff[p] = (uint32_t)(row < nx ? row : nx - 1) * (uint32_t)a.ldx + (((lane & 7) ^ S::fx(row)) << 4);
+  }
+#pragma unroll
+  for (int p = 0; p < S::kQP; ++p) {
+    const int row = (wave * S::kQP + p) * 8 + (lane >> 3);
+    qoff[p] = (uint32_t)(row < nq ? row : nq - 1) * (uint32_t)a.ldq + (((lane & 7) ^ (row & 7)) << 4);
+  }
+  const uint8_t* xb = uniform(a.x + n0 * a.ldx);
+  const uint8_t* qb = uniform(a.q + m0 * a.ldq);
+  const float* xsb = uniform(a.xs + (TILE ? n0 / kBlock : n0));
+  const float* qsb = uniform(a.qs + m0);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  auto stage = [&](int b, int buf) __attribute__((always_inline)) {
+    const uint32_t at = lds0 + buf * S::kStage;
+    const uint8_t* x = xb + (int64_t)b * kBlock;
+    const uint8_t* q = qb + (int64_t)b * kBlock;
+#pragma unroll
+    for (int p = 0; p < S::kXP; ++p) lds_dma<16>(at + (wave * S::kXP + p) * 1024, xoff[p], x);
+#pragma unroll
+    for (int p = 0; p < S::kQP; ++p) lds_dma<16>(at + S::kX + (wave * S::kQP + p) * 1024, qoff[p], q);
+    // (every wave issues the same number, so that one count waits for a stage: the last pieces may repeat)
+#pragma unroll
+    for (int j = 0; j < S::kSP; ++j) {
+      const int i = (j * S::kWaves + wave) % ((S::TN + S::TM) / 64);
+      if (i < S::TN / 64) {
+        const int row = i * 64 + lane, n = row < nx ? row : nx - 1;
+        lds_dma<4>(at + S::kX + S::kQ + i * 256, (uint32_t)(TILE ? n / kBlock : n) * 4, xsb + b * a.ldxs);
+      } else {
+        const int row = (i - S::TN / 64) * 64 + lane;
+        lds_dma<4>(at + S::kX + S::kQ + i * 256, (uint32_t)(row < nq ? row : nq - 1) * 4, qsb + b * a.ldqs);
+      }
+    }
+  };
+
+  // this lane's places in a stage
+  uint32_t xat[4], qat;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int row = wn * 64 + (t / V) * 16 * V + (r >> 2) * 4 * V + (t % V) * 4 + (r & 3);
+    xat[t] = row * kBlock + ((g ^ S::fx(row)) << 4);
+  }
+  qat = S::kX + (wm * MT * 16 + r) * kBlock + ((g ^ (r & 7)) << 4);
+
+  f32x4 acc[MT][4] = {};
+  // D stages: while block b is computed, blocks b + 1 .. b + D - 1 are in flight.  (Past the last block
+  // the last one is loaded again, into a stage that nobody reads, so that the count stays the same.)
+  auto at_most = [&](int b) { return b < a.kb ? b : a.kb - 1; };
+#pragma unroll
+  for (int i = 0; i < D - 1; ++i) stage(at_most(i), i);
+  int cur = 0;
+  for (int b = 0; b < a.kb; ++b) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * S::kLoads) : "memory");
+    __syncthreads();  // block b is in for every wave, and the stage of block b - 1 is free
+    stage(at_most(b + D - 1), cur == 0 ? D - 1 : cur - 1);
+    const char* at = smem + cur * S::kStage;
+    cur = cur + 1 == D ? 0 : cur + 1;
+    const float* sc = (const float*)(at + S::kX + S::kQ);
+    typedef typename Mode<T>::Frag Frag;
+    Frag x[4], q;
+    f32x4 sx[4], p[3];
+    float sq[MT];
+    auto load_q = [&](int mt) __attribute__((always_inline)) {
+      const char* qp = at + mt * 16 * kBlock;
+      return Mode<T>::make(*(const u32x4*)(qp + qat), *(const u32x4*)(qp + (qat ^ 64)));
+    };
+    q = load_q(0);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) x[t] = Mode<T>::make(*(const u32x4*)(at + xat[t]), *(const u32x4*)(at + (xat[t] ^ 64)));
+    float s1 = 0.f;
+    if constexpr (TILE) s1 = sc[wn * 64];  // (64 items of one tile)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) sq[mt] = sc[S::TN + wm * MT * 16 + mt * 16 + r];
+    if constexpr (!TILE) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) sx[t] = *(const f32x4*)(sc + wn * 64 + (t / V) * 16 * V + g * 4 * V + (t % V) * 4);
+    }
+    // product i is scaled and added two products later, when it is ready
+    auto add = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float f = TILE ? sq[i / 4] : sq[i / 4] * sx[i % 4][j];
+        acc[i / 4][i % 4][j] = fmaf(f, p[i % 3][j], acc[i / 4][i % 4][j]);
+      }
+    };
+    if constexpr (TILE) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sq[mt] *= s1;
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      Frag qn = q;
+      if (mt + 1 < MT) qn = load_q(mt + 1);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int i = mt * 4 + t;
+        p[i % 3] = Mode<T>::dot(x[t], q);
+        if (i >= 2) add(i - 2);
+      }
+      q = qn;
+    }
+    add(MT * 4 - 2);
+    add(MT * 4 - 1);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+
+  // The results are turned around in the LDS (all reads of the stages are done), so that a store covers
+  // 1 KiB of the tile's score rows, each row's part whole: full lines but for a row's two ends.
+  constexpr int kRow = S::TN * (int)sizeof(T), kChunks = kRow / 16;  // bytes and 16-byte chunks of a row
+  constexpr int kSwz = kChunks < 16 ? kChunks - 1 : 15;
+  static_assert(kChunks <= 64, "a store covers whole rows");
+  typedef T Out __attribute__((ext_vector_type(4 * V)));
+  typedef T OutAt __attribute__((ext_vector_type(4 * V), aligned(sizeof(T))));
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    char* row = smem + (wm * MT * 16 + mt * 16 + r) * kRow;
+#pragma unroll
+    for (int u = 0; u < 4 / V; ++u) {
+      Out v;
+#pragma unroll
+      for (int j = 0; j < 4 * V; ++j) v[j] = (T)acc[mt][u * V + (j >> 2)][j & 3];
+      *(Out*)(row + (((wn * 16 / V + u * 4 + g) ^ (r & kSwz)) << 4)) = v;
+    }
+  }
+  __syncthreads();
+  const int c = threadIdx.x & (kChunks - 1);
+  const int64_t n = n0 + c * 4 * V;
+  if (n >= a.N) return;
+#pragma unroll
+  for (int i = 0; i < S::TM * kChunks / S::kThreads; ++i) {
+    const int row = i * (S::kThreads / kChunks) + threadIdx.x / kChunks;
+    const int64_t m = m0 + row;
+    if (m >= a.M) break;
+    const Out v = *(const Out*)(smem + row * kRow + ((c ^ (row & kSwz)) << 4));
+    T* p = (T*)a.out + m * a.ldo + n;
+    if (n + 4 * V <= a.N) {
+      __builtin_nontemporal_store(OutAt(v), (OutAt*)p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4 * V; ++j)
+        if (n + j < a.N) p[j] = v[j];
+    }
+  }
+}
+
+// ---- which kernel ---------------------------------------------------------------------------
+int too_many() { return abi_fail(BB_E_ARG, "bb_scores_fp8: too many scores for one call"); }
+
+template <typename T, int KS, int PF>
+int launch_few(const ProductArgs& a, void* stream) {
+  const int64_t n_groups = (a.N + 15) / 16, total = n_groups * ((a.M + 15) / 16);
+  if (total > (int64_t)(0xFFFFFFFFu / (KS * 64))) return too_many();
+  return abi_launch("bb_scores_fp8", product_few_kernel<T, 1, 1, KS, PF>, dim3((uint32_t)total), dim3(KS * 64), 0,
+                    (hipStream_t)stream, a, (int)n_groups);
+}
+
+template <typename T, int WN, int WM, int MT, int D>
+int launch_tile(const ProductArgs& a, void* stream) {
+  using S = TileShape<T, WN, WM, MT, D>;
+  const int64_t tiles_m = (a.M + S::TM - 1) / S::TM, tiles_n = (a.N + S::TN - 1) / S::TN;
+  if (tiles_m * tiles_n > (int64_t)(0xFFFFFFFFu / S::kThreads)) return too_many();
+  return abi_launch("bb_scores_fp8", a.tile ? product_tile_kernel<T, true, WN, WM, MT, D> : product_tile_kernel<T, false, WN, WM, MT, D>,
+                    dim3((uint32_t)(tiles_m * tiles_n)), dim3(S::kThreads), 0, (hipStream_t)stream, a, (int)tiles_m,
+                    (int)tiles_n);
+}
+
+inline int64_t tiles(const ProductArgs& a, int t) { return ((a.M + t - 1) / t) * ((a.N + t - 1) / t); }
+inline int64_t up(int64_t x, int64_t by) { return (x + by - 1) / by; }
+
+template <typename T>
+int launch_product(const ProductArgs& a, void* stream) {
+  // The tiles' source offsets are 32-bit within 256 rows.
+  const bool far = a.ldx >= (1 << 24) || a.ldq >= (1 << 24);
+  if (a.M <= 16 || far) {
+    // one block a wave while it is short (3 blocks, 25,216 items, 1 query: 4.1 us against 8.3 with 8 waves and
+    // 6.2 with one), longer rows split over more waves (32 blocks, 8,192 items, 16 queries: 12.1 us against 13.3)
+    return a.kb == 1 ? launch_few<T, 1, 1>(a, stream) : a.kb <= 8 ? launch_few<T, 4, 1>(a, stream) : launch_few<T, 8, 2>(a, stream);
+  }
+  if (tiles(a, 128) < 200) return launch_tile<T, 1, 4, 1, 3>(a, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (21 * up(tiles(a, 256), 256) <= 11 * up(tiles(a, 128), 512)) return launch_tile<T, 4, 2, 8, 2>(a, stream);
+  }
+  return launch_tile<T, 2, 2, 4, 2>(a, stream);
 }
 
 int check_rows(const bb_fp8_rows* r, const std::string& what) {
@@ -344,14 +662,7 @@ extern "C" int bb_scores_fp8(int32_t device, const bb_fp8_rows* q, const bb_fp8_
     if ((rc = dev.enter(device, "bb_scores_fp8"))) return rc;
     ProductArgs a{q->codes, items->codes, q->scales, items->scales, q->ld, items->ld, q->scales_ld, items->scales_ld,
                   out, ldo, q->rows, items->rows, (int32_t)blocks_of(q->d), items->tile != 0};
-    const int64_t n_groups = (a.N + 255) / 256, m_groups = (a.M + 15) / 16;
-    if (n_groups * m_groups > 0xFFFFFFFFll / 256) return bad("too many scores for one call");
-    auto go = [&](auto kernel) {
-      return abi_launch("bb_scores_fp8", kernel, dim3((uint32_t)(n_groups * m_groups)), dim3(256), 0,
-                        (hipStream_t)stream, a, (int)n_groups);
-    };
-    if (dtype == BB_F32) return go(product_kernel<float>);
-    if (dtype == BB_BF16) return go(product_kernel<__bf16>);
-    return go(product_kernel<_Float16>);
+    return dtype == BB_F32 ? launch_product<float>(a, stream) : dtype == BB_BF16 ? launch_product<__bf16>(a, stream)
+                                                                         : launch_product<_Float16>(a, stream);
   });
 }

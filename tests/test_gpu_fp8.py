@@ -71,11 +71,14 @@ def test_quantize_special_values(br, tile):
     assert torch.equal(got.codes.cpu().float(), codes.float())
     assert torch.equal(torch.nan_to_num(got.scales.cpu(), nan=-1.0), torch.nan_to_num(scales, nan=-1.0))
     assert torch.isnan(scales).any()
-    # a score that reads such a block is NaN, every other one is not
+    # a score that reads such a block is NaN, every other one is not; but for row 2, whose blocks' sums
+    # are 3e38 times the sum of 128 query values: past f32's 3.4e38 as soon as those sum to 1.14, with either
+    # sign, so that infinities of both signs may meet in any order of the blocks
     q = br.quantize_rows(make(4, 400).to(DEV))
     nan = torch.isnan(br.scores_fp8(q, got)).cpu()
     bad = torch.isnan(scales).any(0)
     bad = bad.repeat_interleave(128)[:300] if tile else bad
+    nan[:, 2] = False
     assert torch.equal(nan, bad[None, :].expand(4, 300))
 
 
