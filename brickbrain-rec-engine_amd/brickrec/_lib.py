@@ -90,6 +90,8 @@ _lib = None
 def load() -> C.CDLL:
     """Load libbrickrec.so once; raise BrickrecError if it is not built."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib

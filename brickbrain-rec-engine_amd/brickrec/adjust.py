@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib as L
-from .fp8 import _CODE, _On, _check_out, _ld, _refuse_grad, _rows_of
+from .fp8 import _CODE, _On, _check_out, _ld, _raw_stream, _refuse_grad, _rows_of
 
 Number = Union[float, torch.Tensor]
 
@@ -23,14 +23,22 @@ def mask_words(mask: torch.Tensor) -> torch.Tensor:
     return (pad.to(torch.int64) << bit).sum(-1).to(torch.int32)
 
 
+_IDS = (torch.int32, torch.int64)
+_F32 = (torch.float32,)
+_WORDS = (torch.int32, torch.uint32)
+
+
 def _list(t, name, dtypes, B, dev):
     """A list for each row [B, m], or one for all [m] -> (tensor, entries, elements between rows)."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.device != dev:
-        raise TypeError(f"{name} is a tensor of {' or '.join(str(d) for d in dtypes)} on {dev}")
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != dev:
+        raise TypeError(f"{name} is a tensor of {' or '.join(str(d) for d in dtypes)} on cuda:{dev}")
     if t.dim() == 1:
         return t.contiguous(), t.shape[0], 0
     if t.dim() != 2 or t.shape[0] != B:
         raise ValueError(f"{name} is [{B}, m] or [m]: got {tuple(t.shape)}")
+    if t.is_contiguous():
+        m = t.shape[1]
+        return t, m, m or 1
     if t.stride(0) == 0 and t.stride(1) == 1:  # one list expanded over the rows
         return t, t.shape[1], 0
     t = _rows_of(t)
@@ -40,8 +48,8 @@ def _list(t, name, dtypes, B, dev):
 def _per_row(v: Number, name, B, dev):
     """A value for all rows, or a tensor of one for each -> (pointer or None, value, tensor)."""
     if isinstance(v, torch.Tensor):
-        if v.dtype != torch.float32 or v.device != dev or tuple(v.shape) != (B,):
-            raise TypeError(f"{name} is a number or a float32 tensor [{B}] on {dev}")
+        if v.dtype is not torch.float32 or v.get_device() != dev or v.dim() != 1 or v.shape[0] != B:
+            raise TypeError(f"{name} is a number or a float32 tensor [{B}] on cuda:{dev}")
         v = v.contiguous()
         return v.data_ptr(), 0.0, v
     return None, float(v), None
@@ -64,66 +72,68 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     -1).  seen_len: int32 [B].  repetition (> 0), presence, frequency: numbers, or f32 [B].  bias: f32, as
     bias_ids.  mask: words [⌈n/32⌉] or [B, ⌈n/32⌉] (``ItemIndex.eval_mask_bits``), or bool [n] or [B, n],
     which costs a few launches more.  out: where to write; may be ``scores`` itself."""
-    if not isinstance(scores, torch.Tensor) or scores.device.type != "cuda" or scores.dtype not in _CODE:
+    if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _CODE:
         raise TypeError("scores are a float32, bfloat16 or float16 tensor on a GPU")
     if scores.dim() != 2:
         raise ValueError(f"scores are [B, n]: got {tuple(scores.shape)}")
-    params = (repetition, presence, frequency)
-    tensors = [t for t in (scores, seen, seen_len, bias_ids, bias, mask, out, *params) if isinstance(t, torch.Tensor)]
-    _refuse_grad(*tensors)
-    if not isinstance(repetition, torch.Tensor) and not float(repetition) > 0.0:
-        raise ValueError(f"repetition is above 0: got {repetition}")
+    if stream is not None:
+        with _On(stream, scores.device, (scores, seen, seen_len, repetition, presence, frequency, bias_ids, bias, mask, out)):
+            return adjust_scores(scores, seen=seen, seen_len=seen_len, repetition=repetition, presence=presence,
+                                 frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, out=out)
+    if torch.is_grad_enabled():
+        _refuse_grad(*(t for t in (scores, repetition, presence, frequency, bias) if isinstance(t, torch.Tensor)))
     B, n = scores.shape
-    dev = scores.device
-    a = L.bb_adjust()
-    with _On(stream, dev, tensors) as handle:
-        keep = []
-        if out is None:
-            scores = _rows_of(scores)
-            out = torch.empty((B, n), dtype=scores.dtype, device=dev)
-        else:
-            _check_out(out, (B, n), scores.dtype, dev)
-            scores = _rows_of(scores)
-        a.scores, a.out, a.B, a.n, a.ld_scores, a.ld_out = scores.data_ptr(), out.data_ptr(), B, n, _ld(scores), _ld(out)
-        a.dtype = _CODE[scores.dtype]
-        if seen is not None:
-            t, a.n_seen, a.ld_seen = _list(seen, "seen", (torch.int32, torch.int64), B, dev)
-            a.seen = t.data_ptr()
-            a.ids64 |= int(t.dtype == torch.int64)
-            keep.append(t)
-            if seen_len is not None:
-                if seen_len.dtype != torch.int32 or seen_len.device != dev or tuple(seen_len.shape) != (B,):
-                    raise TypeError(f"seen_len is an int32 tensor [{B}] on {dev}")
-                seen_len = seen_len.contiguous()
-                a.seen_len = seen_len.data_ptr()
-            a.repetition, a.repetition_all, t0 = _per_row(repetition, "repetition", B, dev)
-            a.presence, a.presence_all, t1 = _per_row(presence, "presence", B, dev)
-            a.frequency, a.frequency_all, t2 = _per_row(frequency, "frequency", B, dev)
-            keep += [t0, t1, t2]
-        elif seen_len is not None:
-            raise ValueError("seen_len without seen")
-        if (bias_ids is None) != (bias is None):
-            raise ValueError("bias_ids and bias come together")
-        if bias_ids is not None:
-            if bias.shape != bias_ids.shape:
-                raise ValueError(f"bias is as bias_ids: got {tuple(bias.shape)} and {tuple(bias_ids.shape)}")
-            t, a.n_bias, a.ld_bias = _list(bias_ids, "bias_ids", (torch.int32, torch.int64), B, dev)
-            v, _, ld = _list(bias, "bias", (torch.float32,), B, dev)
-            if ld != a.ld_bias:  # (the two lists share one distance between rows)
-                t, v = t.contiguous(), v.contiguous()
-                a.ld_bias = 0 if t.dim() == 1 else _ld(t)
-            a.bias_ids, a.bias = t.data_ptr(), v.data_ptr()
-            a.ids64 |= 2 * int(t.dtype == torch.int64)
-            keep += [t, v]
-        if mask is not None:
-            if mask.dtype == torch.bool:
-                if mask.shape[-1] != n:
-                    raise ValueError(f"a bool mask is [{n}] or [{B}, {n}]: got {tuple(mask.shape)}")
-                mask = mask_words(mask)
-            t, w, a.ld_mask = _list(mask, "mask", (torch.int32, torch.uint32), B, dev)
-            if w != (n + 31) // 32:
-                raise ValueError(f"the mask of {n} scores has {(n + 31) // 32} words: got {w}")
-            a.mask = t.data_ptr()
-            keep.append(t)
-        L.check(L.load().bb_adjust_scores(dev.index, C.byref(a), handle), "bb_adjust_scores")
+    dev = scores.get_device()
+    scores = _rows_of(scores)
+    if out is None:
+        out = torch.empty((B, n), dtype=scores.dtype, device=scores.device)
+        ld = max(1, n)
+    else:
+        _check_out(out, (B, n), scores.dtype, scores.device)
+        ld = _ld(out)
+    # every tensor that the launch reads has a name here until it is out
+    seen_p = seen_len_p = rep_p = pre_p = fre_p = bias_ids_p = bias_p = mask_p = None
+    n_seen = ld_seen = n_bias = ld_bias = ld_mask = ids64 = 0
+    rep, pre, fre = 1.0, 0.0, 0.0
+    if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
+        raise ValueError(f"repetition is above 0: got {repetition}")
+    if seen is not None:
+        seen, n_seen, ld_seen = _list(seen, "seen", _IDS, B, dev)
+        seen_p, ids64 = seen.data_ptr(), int(seen.dtype is torch.int64)
+        if seen_len is not None:
+            if seen_len.dtype is not torch.int32 or seen_len.get_device() != dev or seen_len.dim() != 1 or seen_len.shape[0] != B:
+                raise TypeError(f"seen_len is an int32 tensor [{B}] on cuda:{dev}")
+            seen_len = seen_len.contiguous()
+            seen_len_p = seen_len.data_ptr()
+        rep_p, rep, repetition = _per_row(repetition, "repetition", B, dev)
+        pre_p, pre, presence = _per_row(presence, "presence", B, dev)
+        fre_p, fre, frequency = _per_row(frequency, "frequency", B, dev)
+    elif seen_len is not None:
+        raise ValueError("seen_len without seen")
+    if (bias_ids is None) != (bias is None):
+        raise ValueError("bias_ids and bias come together")
+    if bias_ids is not None:
+        bias_ids, n_bias, ld_bias = _list(bias_ids, "bias_ids", _IDS, B, dev)
+        bias, m, ld_v = _list(bias, "bias", _F32, B, dev)
+        if bias.dim() != bias_ids.dim() or m != n_bias:
+            raise ValueError(f"bias is as bias_ids: got {tuple(bias.shape)} and {tuple(bias_ids.shape)}")
+        if ld_v != ld_bias:  # (the two lists share one distance between rows)
+            bias_ids, bias = bias_ids.contiguous(), bias.contiguous()
+            ld_bias = _ld(bias_ids)
+        bias_ids_p, bias_p = bias_ids.data_ptr(), bias.data_ptr()
+        ids64 |= 2 * int(bias_ids.dtype is torch.int64)
+    if mask is not None:
+        if mask.dtype is torch.bool:
+            if mask.shape[-1] != n:
+                raise ValueError(f"a bool mask is [{n}] or [{B}, {n}]: got {tuple(mask.shape)}")
+            mask = mask_words(mask)
+        mask, w, ld_mask = _list(mask, "mask", _WORDS, B, dev)
+        if w != (n + 31) // 32:
+            raise ValueError(f"the mask of {n} scores has {(n + 31) // 32} words: got {w}")
+        mask_p = mask.data_ptr()
+    a = L.bb_adjust(scores.data_ptr(), out.data_ptr(), B, n, _ld(scores), ld, _CODE[scores.dtype], ids64, seen_p, n_seen,
+                    ld_seen, seen_len_p, rep_p, pre_p, fre_p, rep, pre, fre, bias_ids_p, bias_p, n_bias, ld_bias, mask_p, ld_mask)
+    rc = L.load().bb_adjust_scores(dev, C.byref(a), _raw_stream(dev))
+    if rc:
+        L.check(rc, "bb_adjust_scores")
     return out

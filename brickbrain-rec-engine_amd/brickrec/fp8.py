@@ -29,38 +29,36 @@ def _refuse_grad(*tensors):
         raise ValueError("no gradient flows through this call: detach the inputs or call it under torch.no_grad()")
 
 
-class _On:
-    """The stream of a call (``handle``).  With a stream of the caller's, outputs are made for it and
-    the inputs' memory is kept from reuse until it has passed this call."""
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream, without the object (2 us a call)
 
-    __slots__ = ("stream", "device", "handle", "_ctx")
+
+class _On:
+    """A stream of the caller's for one call: outputs are made for it, and the inputs' memory is kept
+    from reuse until it has passed the call."""
+
+    __slots__ = ("handle", "_ctx")
 
     def __init__(self, stream, device, inputs):
-        self.stream, self.device, self._ctx = stream, device, None
-        if stream is None:
-            self.handle = torch.cuda.current_stream(device).cuda_stream
-            return
         if stream.device != device:
             raise ValueError(f"stream of {stream.device} for tensors of {device}")
-        self.handle = stream.cuda_stream
-        if stream != torch.cuda.current_stream(device):
+        self.handle, self._ctx = stream.cuda_stream, torch.cuda.stream(stream)
+        if self.handle != _raw_stream(device.index):
             for t in inputs:
-                if t is not None:
+                if isinstance(t, torch.Tensor):
                     t.record_stream(stream)
-            self._ctx = torch.cuda.stream(stream)
 
     def __enter__(self):
-        if self._ctx is not None:
-            self._ctx.__enter__()
+        self._ctx.__enter__()
         return self.handle
 
     def __exit__(self, *exc):
-        if self._ctx is not None:
-            self._ctx.__exit__(*exc)
+        self._ctx.__exit__(*exc)
 
 
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
     """x with its columns next to each other and its rows apart (copied where they are not)."""
+    if x.is_contiguous():
+        return x
     n, d = x.shape
     if (d > 1 and x.stride(1) != 1) or (n > 1 and x.stride(0) < d):
         return x.contiguous()
@@ -68,6 +66,7 @@ def _rows_of(x: torch.Tensor) -> torch.Tensor:
 
 
 def _ld(x: torch.Tensor) -> int:
+    """Elements between the rows of x."""
     return x.stride(0) if x.shape[0] > 1 else max(1, x.shape[1])
 
 
@@ -79,26 +78,38 @@ class Fp8Rows:
     __slots__ = ("codes", "scales", "d", "tile", "_c")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int, tile: bool = False):
-        if codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32:
+        if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32:
             raise TypeError(f"codes are float8_e4m3fn and scales float32: got {codes.dtype} and {scales.dtype}")
-        if codes.device.type != "cuda" or scales.device != codes.device:
+        if not codes.is_cuda or scales.get_device() != codes.get_device():
             raise TypeError("codes and scales are tensors of one GPU")
-        n, kb = codes.shape[0], blocks_of(d)
-        if d < 0 or codes.dim() != 2 or codes.shape[1] != kb * BLOCK:
+        if d < 0 or codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError("codes and scales are matrices")
+        (n, w), (sk, sn), kb = codes.shape, scales.shape, (d + 127) // 128
+        if w != kb * BLOCK:
             raise ValueError(f"codes of rows {d} wide are [n, {kb * BLOCK}]: got {tuple(codes.shape)}")
-        if tuple(scales.shape) != (kb, blocks_of(n) if tile else n):
-            raise ValueError(f"scales of {n} rows {d} wide are [{kb}, {blocks_of(n) if tile else n}]: got {tuple(scales.shape)}")
-        if (n > 0 and kb > 0) and (codes.stride(1) != 1 or (scales.shape[1] > 1 and scales.stride(1) != 1)):
-            raise ValueError("codes and scales are contiguous along their rows")
+        want = (n + 127) // 128 if tile else n
+        if sk != kb or sn != want:
+            raise ValueError(f"scales of {n} rows {d} wide are [{kb}, {want}]: got {tuple(scales.shape)}")
+        ld, sld = w, sn
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            if n > 0 and kb > 0 and (codes.stride(1) != 1 or (sn > 1 and scales.stride(1) != 1)):
+                raise ValueError("codes and scales are contiguous along their rows")
+            ld, sld = _ld(codes), _ld(scales)
         self.codes, self.scales, self.d, self.tile = codes, scales, d, bool(tile)
-        self._c = L.bb_fp8_rows(codes.data_ptr(), scales.data_ptr(), n, d, _ld(codes), _ld(scales), int(self.tile))
+        self._c = L.bb_fp8_rows(codes.data_ptr(), scales.data_ptr(), n, d, ld, sld, 1 if tile else 0)
 
     @classmethod
     def empty(cls, n: int, d: int, tile: bool = False, device=None) -> "Fp8Rows":
+        """Rows to be written (``quantize_rows(..., out=...)``)."""
         dev = torch.device("cuda" if device is None else device)
-        kb = blocks_of(d)
-        return cls(torch.empty((n, kb * BLOCK), dtype=torch.float8_e4m3fn, device=dev),
-                   torch.empty((kb, blocks_of(n) if tile else n), dtype=torch.float32, device=dev), d, tile)
+        kb = (d + 127) // 128
+        sn = (n + 127) // 128 if tile else n
+        new = cls.__new__(cls)
+        new.codes = torch.empty((n, kb * BLOCK), dtype=torch.float8_e4m3fn, device=dev)
+        new.scales = torch.empty((kb, sn), dtype=torch.float32, device=dev)
+        new.d, new.tile = d, bool(tile)
+        new._c = L.bb_fp8_rows(new.codes.data_ptr(), new.scales.data_ptr(), n, d, max(1, kb * BLOCK), max(1, sn), 1 if tile else 0)
+        return new
 
     def __len__(self) -> int:
         return self.codes.shape[0]
@@ -128,20 +139,25 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
     One scale for each block of 128 columns of a row, or with ``tile`` for each 128 × 128 block; a
     block with an infinity or a NaN gets scale NaN and codes 0.  ``out``: rows of the same shape to
     write into."""
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or x.dtype not in _CODE:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _CODE:
         raise TypeError("rows are a float32, bfloat16 or float16 tensor on a GPU")
     if x.dim() != 2:
         raise ValueError(f"rows are [n, d]: got {tuple(x.shape)}")
-    _refuse_grad(x)
-    with _On(stream, x.device, (x,) if out is None else (x, out.codes, out.scales)) as handle:
-        x = _rows_of(x)
-        n, d = x.shape
-        if out is None:
-            out = Fp8Rows.empty(n, d, tile, x.device)
-        elif (len(out), out.d, out.tile, out.device) != (n, d, bool(tile), x.device):
-            raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
-        L.check(L.load().bb_quantize_fp8(x.device.index, x.data_ptr(), _CODE[x.dtype], _ld(x), C.byref(out._c), handle),
-                "bb_quantize_fp8")
+    if x.requires_grad:
+        _refuse_grad(x)
+    if stream is not None:
+        with _On(stream, x.device, (x,) if out is None else (x, out.codes, out.scales)):
+            return quantize_rows(x, tile=tile, out=out)
+    x = _rows_of(x)
+    n, d = x.shape
+    dev = x.get_device()
+    if out is None:
+        out = Fp8Rows.empty(n, d, tile, x.device)
+    elif (len(out), out.d, out.tile, out.codes.get_device()) != (n, d, bool(tile), dev):
+        raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
+    rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), C.byref(out._c), _raw_stream(dev))
+    if rc:
+        L.check(rc, "bb_quantize_fp8")
     return out
 
 
@@ -151,19 +167,25 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     rounded once to ``dtype`` (f32, bf16 or f16).  The queries' scales are per row; the items' per
     row or per tile.  ``out``: a tensor of that shape (its dtype is then the scores') to write into; its
     rows may be strided, columns behind them stay as they were."""
-    dev = queries.codes.device
-    if items.codes.device != dev:
+    q, x = queries.codes, items.codes
+    dev = q.get_device()
+    if x.get_device() != dev:
         raise ValueError("queries and items are on one device")
-    inputs = () if stream is None else (queries.codes, queries.scales, items.codes, items.scales, out)
-    with _On(stream, dev, inputs) as handle:
-        if out is None:
-            if dtype not in _CODE:
-                raise TypeError(f"scores are float32, bfloat16 or float16: not {dtype}")
-            out = torch.empty((queries.codes.shape[0], items.codes.shape[0]), dtype=dtype, device=dev)
-        else:
-            _check_out(out, (queries.codes.shape[0], items.codes.shape[0]), None, dev)
-        L.check(L.load().bb_scores_fp8(dev.index, C.byref(queries._c), C.byref(items._c), out.data_ptr(),
-                                       _CODE[out.dtype], _ld(out), handle), "bb_scores_fp8")
+    if stream is not None:
+        with _On(stream, q.device, (q, queries.scales, x, items.scales, out)):
+            return scores_fp8(queries, items, dtype=dtype, out=out)
+    if out is None:
+        if dtype not in _CODE:
+            raise TypeError(f"scores are float32, bfloat16 or float16: not {dtype}")
+        out = torch.empty((q.shape[0], x.shape[0]), dtype=dtype, device=q.device)
+        ld = max(1, x.shape[0])
+    else:
+        _check_out(out, (q.shape[0], x.shape[0]), None, q.device)
+        ld = _ld(out)
+    rc = L.load().bb_scores_fp8(dev, C.byref(queries._c), C.byref(items._c), out.data_ptr(), _CODE[out.dtype], ld,
+                                _raw_stream(dev))
+    if rc:
+        L.check(rc, "bb_scores_fp8")
     return out
 
 
