@@ -97,6 +97,8 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     rep, pre, fre = 1.0, 0.0, 0.0
     if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
         raise ValueError(f"repetition is above 0: got {repetition}")
+    if seen is not None and bias_ids is not None and {seen.dtype, bias_ids.dtype} == set(_IDS):
+        seen, bias_ids = seen.to(torch.int64), bias_ids.to(torch.int64)  # (the lists of one call have ids of one size)
     if seen is not None:
         seen, n_seen, ld_seen = _list(seen, "seen", _IDS, B, dev)
         seen_p, ids64 = seen.data_ptr(), int(seen.dtype is torch.int64)
@@ -121,7 +123,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
             bias_ids, bias = bias_ids.contiguous(), bias.contiguous()
             ld_bias = _ld(bias_ids)
         bias_ids_p, bias_p = bias_ids.data_ptr(), bias.data_ptr()
-        ids64 |= 2 * int(bias_ids.dtype is torch.int64)
+        ids64 = int(bias_ids.dtype is torch.int64)
     if mask is not None:
         if mask.dtype is torch.bool:
             if mask.shape[-1] != n:

@@ -1,11 +1,11 @@
 // adjust.hip — penalties for ids seen already, sparse biases and a bit mask on dense scores
 // (bb_adjust_scores).
 //
-// One pass over the scores.  A workgroup takes one chunk of one row: it counts the row's seen
-// ids that fall into the chunk in LDS (integer atomics: the order does not matter), keeps the
-// position of the last bias entry of each id there (integer max), and then streams the chunk,
-// every thread one group of 8 scores at a time.  The row's lists are read again by every chunk of
-// the row, from the L2: 4 bytes an entry against 2 x 4096 scores moved.
+// One pass over the scores, bound by moving them.  A workgroup takes one chunk of one row.  Its scores
+// and mask bits are loaded first; while they are on their way, the row's lists are read (from the L2: every
+// chunk of a row reads them again, so long lists get larger chunks) and what concerns the chunk is
+// kept in LDS, one word a score: the position of the last bias entry of the id in the high half,
+// how often it was seen in the low half.  Integer maxima and sums, so their order does not matter.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -16,78 +16,118 @@
 namespace bb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kVec = 8;        // scores per thread and step: 16 bytes of a 16-bit type, a byte of the mask
-constexpr int kChunk = 4096;   // scores per workgroup (a multiple of 32: whole mask words)
+constexpr int kVec = 8;  // scores per thread: 16 bytes of a 16-bit type, a byte of the mask
 
-template <typename T>
-struct Vec8 {
-  typedef T type __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+template <typename T, int N>
+struct VecOf {
+  typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
 };
 
-__device__ __forceinline__ int64_t list_id(const void* p, int64_t i, bool wide) {
-  return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
-}
+// A row's list of ids, 4 at a time to a thread; the first 4 are loaded when it is made, so that their
+// latency passes beside that of the scores.
+template <int THREADS, typename Id>
+struct List {
+  typedef typename VecOf<Id, 4>::type V;
+  const Id* ids;
+  int n;
+  V first;
+  __device__ __forceinline__ List(const void* p, int64_t at, int n_) : ids((const Id*)p + at), n(n_) {
+    if ((int)threadIdx.x * 4 + 4 <= n) first = *(const V*)(ids + threadIdx.x * 4);
+  }
+  // f(entry, id) for the first `m` <= n entries
+  template <typename F>
+  __device__ __forceinline__ void each(int m, F&& f) const {
+    for (int i = threadIdx.x * 4; i < m; i += THREADS * 4) {
+      if (i + 4 <= n) {
+        const V v = i < THREADS * 4 ? first : *(const V*)(ids + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j < m) f(i + j, (int64_t)v[j]);
+      } else {
+        for (int j = i; j < m; ++j) f(j, (int64_t)ids[j]);
+      }
+    }
+  }
+};
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void adjust_kernel(bb_adjust a, int n_chunks) {
-  extern __shared__ uint32_t lds[];
+// SPLIT: lists of 2^16 entries or more, whose counts and positions take a word each.
+template <typename T, typename Id, int THREADS, bool SPLIT>
+__global__ __launch_bounds__(THREADS) void adjust_kernel(bb_adjust a, int n_chunks) {
+  constexpr int kChunk = THREADS * kVec;
+  __shared__ __attribute__((aligned(16))) uint32_t lds[kChunk * (SPLIT ? 2 : 1)];
   const int64_t row = blockIdx.x / n_chunks;
   const int64_t c0 = (int64_t)(blockIdx.x % n_chunks) * kChunk;
   const int len = (int)(a.n - c0 < kChunk ? a.n - c0 : kChunk);
-  uint32_t* count = lds;
-  uint32_t* slot = lds + (a.seen ? kChunk : 0);
-  const int n_words = (a.seen ? kChunk : 0) + (a.bias_ids ? kChunk : 0);
-  if (n_words) {
-    for (int i = threadIdx.x; i < n_words; i += kThreads) lds[i] = 0;
-    __syncthreads();
-    if (a.seen) {
-      int64_t h = a.n_seen;
-      if (a.seen_len) {
-        const int64_t l = a.seen_len[row];
-        h = l < 0 ? 0 : l < h ? l : h;
-      }
-      for (int64_t i = threadIdx.x; i < h; i += kThreads) {
-        const uint64_t v = (uint64_t)(list_id(a.seen, row * a.ld_seen + i, a.ids64 & 1) - c0);
-        if (v < (uint64_t)len) atomicAdd(&count[v], 1u);
-      }
-    }
-    if (a.bias_ids) {
-      for (int64_t i = threadIdx.x; i < a.n_bias; i += kThreads) {
-        const uint64_t v = (uint64_t)(list_id(a.bias_ids, row * a.ld_bias + i, a.ids64 & 2) - c0);
-        if (v < (uint64_t)len) atomicMax(&slot[v], (uint32_t)i + 1u);
-      }
-    }
-    __syncthreads();
-  }
-  const float rep = a.repetition ? a.repetition[row] : a.repetition_all;
-  const float pre = a.presence ? a.presence[row] : a.presence_all;
-  const float fre = a.frequency ? a.frequency[row] : a.frequency_all;
   const T* src = (const T*)a.scores + row * a.ld_scores + c0;
   T* dst = (T*)a.out + row * a.ld_out + c0;
   const uint32_t* mask = a.mask ? a.mask + row * a.ld_mask + (c0 >> 5) : nullptr;
-  typedef typename Vec8<T>::type V;
-  auto one = [&](float x, int i) {
-    if (a.seen) {
-      const uint32_t c = count[i];
-      if (c) x = (x > 0.f ? x / rep : x * rep) - (fre * (float)c + pre);
+  typedef typename VecOf<T, kVec>::type V;
+  typedef uint32_t W __attribute__((ext_vector_type(4)));
+  const int i = threadIdx.x * kVec;  // this thread's 8 scores of the chunk
+  V v;
+  uint32_t bits = 0xFFu;
+  if (i < len && mask) bits = mask[i >> 5] >> (i & 31);
+  if (i + kVec <= len) v = *(const V*)(src + i);
+  const float rep = a.repetition ? a.repetition[row] : a.repetition_all;
+  const float pre = a.presence ? a.presence[row] : a.presence_all;
+  const float fre = a.frequency ? a.frequency[row] : a.frequency_all;
+  const bool lists = a.seen || a.bias_ids;
+  if (lists) {
+    const List<THREADS, Id> seen(a.seen, row * a.ld_seen, a.seen ? (int)a.n_seen : 0);
+    const List<THREADS, Id> biased(a.bias_ids, row * a.ld_bias, a.bias_ids ? (int)a.n_bias : 0);
+    int n_seen = seen.n;
+    if (a.seen && a.seen_len) {
+      const int l = a.seen_len[row];
+      n_seen = l < 0 ? 0 : l < n_seen ? l : n_seen;
     }
+#pragma unroll
+    for (int z = 0; z < kChunk * (SPLIT ? 2 : 1) / 4; z += THREADS) *(W*)(lds + (z + threadIdx.x) * 4) = W{0, 0, 0, 0};
+    __syncthreads();
+    uint32_t* slot = SPLIT ? lds + kChunk : lds;
     if (a.bias_ids) {
-      const uint32_t s = slot[i];
-      if (s) x += a.bias[row * a.ld_bias + (s - 1)];
+      biased.each(biased.n, [&](int e, int64_t id) {
+        const uint64_t at = (uint64_t)(id - c0);
+        if (at < (uint64_t)len) atomicMax(&slot[at], SPLIT ? (uint32_t)e + 1u : ((uint32_t)e + 1u) << 16);
+      });
+      if (!SPLIT && a.seen) __syncthreads();  // (the maxima are over words whose counts are still 0)
     }
+    seen.each(n_seen, [&](int, int64_t id) {
+      const uint64_t at = (uint64_t)(id - c0);
+      if (at < (uint64_t)len) atomicAdd(&lds[at], 1u);
+    });
+    __syncthreads();
+  }
+  const float* bias = a.bias_ids ? a.bias + row * a.ld_bias : nullptr;
+  auto one = [&](float x, uint32_t count, uint32_t slot) {
+    if (count) x = (x > 0.f ? x / rep : x * rep) - (fre * (float)count + pre);
+    if (slot) x += bias[slot - 1];
     return x;
   };
-  for (int i = threadIdx.x * kVec; i < len; i += kThreads * kVec) {
-    const uint32_t bits = mask ? mask[i >> 5] >> (i & 31) : 0xFFu;
-    if (i + kVec <= len) {
-      V v = *(const V*)(src + i);
+  auto count_of = [&](uint32_t w) { return SPLIT ? w : w & 0xFFFFu; };
+  if (i + kVec <= len) {
+    if (lists) {
+      uint32_t w[kVec], t[kVec];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) v[j] = (bits >> j) & 1 ? (T)one((float)v[j], i + j) : (T)-__builtin_inff();
-      *(V*)(dst + i) = v;
-    } else {
-      for (int j = 0; i + j < len; ++j)
-        dst[i + j] = (bits >> j) & 1 ? (T)one((float)src[i + j], i + j) : (T)-__builtin_inff();
+      for (int j = 0; j < kVec; j += 4) {
+        *(W*)&w[j] = *(const W*)(lds + i + j);
+        if constexpr (SPLIT) *(W*)&t[j] = *(const W*)(lds + kChunk + i + j);
+      }
+      uint32_t any = 0;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) any |= SPLIT ? w[j] | t[j] : w[j];
+      if (any) {  // (most groups of 8 hold no listed id)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) v[j] = (T)one((float)v[j], count_of(w[j]), SPLIT ? t[j] : w[j] >> 16);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) v[j] = (bits >> j) & 1 ? v[j] : (T)-__builtin_inff();
+    *(V*)(dst + i) = v;
+  } else {
+    for (int j = 0; i + j < len; ++j) {
+      float x = (float)src[i + j];
+      if (lists) x = one(x, count_of(lds[i + j]), SPLIT ? lds[kChunk + i + j] : lds[i + j] >> 16);
+      dst[i + j] = (bits >> j) & 1 ? (T)x : (T)-__builtin_inff();
     }
   }
 }
@@ -98,7 +138,7 @@ int check(const bb_adjust* a) {
   if (!a) return bad("null arguments");
   if (a->dtype != BB_F32 && a->dtype != BB_BF16 && a->dtype != BB_F16) return bad("dtype must be BB_F32, BB_BF16 or BB_F16");
   if (a->B < 0 || a->n < 0) return bad("negative size");
-  if (a->n > 0x7FFFFFFF || a->n_seen > 0x7FFFFFFF || a->n_bias > 0x7FFFFFFF) return bad("n and the lists are below 2^31");
+  if (a->n > 0x7FFFFFFF || a->n_seen >= 1 << 30 || a->n_bias >= 1 << 30) return bad("n is below 2^31, the lists below 2^30");
   if (a->B == 0 || a->n == 0) return BB_OK;
   if (!a->scores || !a->out) return bad("null scores or out");
   if (a->ld_scores < a->n || a->ld_out < a->n) return bad("rows overlap (ld < n)");
@@ -116,11 +156,31 @@ int check(const bb_adjust* a) {
   if (a->seen && a->ld_seen != 0 && a->ld_seen < a->n_seen) return bad("ld_seen < n_seen");
   if (a->bias_ids && a->ld_bias != 0 && a->ld_bias < a->n_bias) return bad("ld_bias < n_bias");
   if (a->mask && a->ld_mask != 0 && a->ld_mask < (a->n + 31) / 32) return bad("ld_mask < ceil(n/32)");
-  const uintptr_t is = a->ids64 & 1 ? 8 : 4, ib = a->ids64 & 2 ? 8 : 4;
-  if ((uintptr_t)a->seen % is || (uintptr_t)a->bias_ids % ib || (uintptr_t)a->seen_len % 4 || (uintptr_t)a->bias % 4 ||
+  const uintptr_t ib = a->ids64 ? 8 : 4;
+  if ((uintptr_t)a->seen % ib || (uintptr_t)a->bias_ids % ib || (uintptr_t)a->seen_len % 4 || (uintptr_t)a->bias % 4 ||
       (uintptr_t)a->mask % 4 || (uintptr_t)a->repetition % 4 || (uintptr_t)a->presence % 4 || (uintptr_t)a->frequency % 4)
     return bad("a list, mask or parameter is not aligned to its type");
   return BB_OK;
+}
+
+template <typename T, typename Id, int THREADS, bool SPLIT>
+int launch(const bb_adjust& a, void* stream) {
+  constexpr int kChunk = THREADS * kVec;
+  const int64_t n_chunks = (a.n + kChunk - 1) / kChunk;
+  // a launch holds less than 2^32 threads
+  if (a.B > (int64_t)(0xFFFFFFFFu / THREADS) / n_chunks) return abi_fail(BB_E_ARG, "bb_adjust_scores: too many rows for one call");
+  return abi_launch("bb_adjust_scores", adjust_kernel<T, Id, THREADS, SPLIT>, dim3((uint32_t)(a.B * n_chunks)),
+                    dim3(THREADS), 0, (hipStream_t)stream, a, (int)n_chunks);
+}
+
+template <typename T, typename Id>
+int launch_type(const bb_adjust& a, void* stream) {
+  if (a.n_seen >= 1 << 16 || a.n_bias >= 1 << 16) return launch<T, Id, 1024, true>(a, stream);
+  // Longer lists are read by fewer, larger workgroups: 64 rows of 131,072 bf16 with 4,096 ids each take 15.8 us with
+  // 256 threads and 13.3 with 1024; 256 rows of 25,216 f32 with 200 ids 12.3 and 14.9 (copying those
+  // scores alone: 7.1 and 11.0 us at the 4.7 TB/s of a large copy).  One row of 25,216: 3.7 us.
+  if (a.n_seen + a.n_bias > 1024) return launch<T, Id, 1024, false>(a, stream);
+  return launch<T, Id, 256, false>(a, stream);
 }
 
 }  // namespace
@@ -134,19 +194,14 @@ extern "C" int bb_adjust_scores(int32_t device, const bb_adjust* args, void* str
     bb_adjust a = *args;
     if (a.n_seen == 0) a.seen = nullptr;
     if (a.n_bias == 0) a.bias_ids = nullptr;
-    const int64_t n_chunks = (a.n + kChunk - 1) / kChunk;
-    // a launch holds less than 2^32 threads
-    if (a.B > (int64_t)(0xFFFFFFFFu / kThreads) / n_chunks)
-      return abi_fail(BB_E_ARG, "bb_adjust_scores: too many rows for one call");
     CallDevice dev;
     if ((rc = dev.enter(device, "bb_adjust_scores"))) return rc;
-    const uint32_t lds = ((a.seen ? kChunk : 0) + (a.bias_ids ? kChunk : 0)) * 4;
-    const dim3 grid((uint32_t)(a.B * n_chunks));
-    auto go = [&](auto kernel) {
-      return abi_launch("bb_adjust_scores", kernel, grid, dim3(kThreads), lds, (hipStream_t)stream, a, (int)n_chunks);
+    auto go = [&](auto id) {
+      using Id = decltype(id);
+      return a.dtype == BB_F32 ? launch_type<float, Id>(a, stream)
+             : a.dtype == BB_BF16 ? launch_type<__bf16, Id>(a, stream)
+                                  : launch_type<_Float16, Id>(a, stream);
     };
-    if (a.dtype == BB_F32) return go(adjust_kernel<float>);
-    if (a.dtype == BB_BF16) return go(adjust_kernel<__bf16>);
-    return go(adjust_kernel<_Float16>);
+    return a.ids64 ? go(int64_t{}) : go(int32_t{});
   });
 }

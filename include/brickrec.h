@@ -316,7 +316,7 @@ int bb_scores_fp8(int32_t device, const bb_fp8_rows* q, const bb_fp8_rows* items
  *   c > 0:  s = (s > 0 ? s / repetition : s * repetition) - (frequency * c + presence)
  *   s += the bias of v, if the row's bias list holds v (the last entry where it does so twice)
  *   s = -infinity where the mask's bit v is 0, whatever s was (NaN too)
- * Ids outside [0, n) are skipped (lists padded with -1). */
+ * Ids outside [0, n) are skipped (lists padded with -1).  n is below 2^31, the lists below 2^30. */
 typedef struct {
   const void* scores;        /* B x n of `dtype`, ld_scores elements between rows            */
   void* out;                 /* the same shape and type, ld_out between rows; may be scores
@@ -324,7 +324,7 @@ typedef struct {
   int64_t B, n;
   int64_t ld_scores, ld_out;
   int32_t dtype;             /* BB_F32 / BB_BF16 / BB_F16                                    */
-  int32_t ids64;             /* bit 0: seen is int64, bit 1: bias_ids is int64 (int32 if not)*/
+  int32_t ids64;             /* the ids of both lists are int64 (0: int32)                   */
   const void* seen;          /* B x n_seen ids, ld_seen between rows (0: one list for all);
                                 NULL = none                                                  */
   int64_t n_seen, ld_seen;

@@ -94,6 +94,8 @@ def test_id_types_and_shared_lists(br, ids):
     far = a["seen"].clone().to(torch.int64)
     far[:, 0], far[:, 1] = 2 ** 40, -2 ** 40         # far outside [0, n): skipped
     check({**a, "seen": far}, run(br, {**a, "seen": far}))
+    mixed = {**a, "seen": a["seen"].to(torch.int32), "bias_ids": a["bias_ids"].to(torch.int64)}
+    check(mixed, run(br, mixed))
     b = {**a, "seen": a["seen"][0], "bias_ids": a["bias_ids"][1], "bias": a["bias"][1], "repetition": 1.5, "presence": 0.0}
     check(b, run(br, b))
     c = {**b, "seen": b["seen"].expand(4, 50)}
@@ -126,6 +128,19 @@ def test_in_place_strided_and_misaligned(br, dtype, n):
     got = br.adjust_scores(a["scores"].t().contiguous().to(DEV).t(), mask=words[:, 1:-2],
                            **{**dev, "seen": wide[:, :30], "bias_ids": wb[:, 4:10]})
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("H, nb", [(70000, 3), (5, 70000), (65535, 65535), (0, 65536), (65536, 0)])
+def test_lists_at_and_past_16_bits(br, H, nb):
+    n = 9000
+    a = make(2, n, torch.float32, H, nb, seed=H + nb)
+    if H:
+        a["seen"][0] = 7                              # one id in every entry
+        a["seen_len"] = torch.tensor([H, H - 1], dtype=torch.int32)
+        a["frequency"] = torch.tensor([0.5, 0.25])
+    if nb:
+        a["bias_ids"][1] = 8                          # the last of all entries counts
+    check(a, run(br, a))
 
 
 def test_mask_words_layout(br):
