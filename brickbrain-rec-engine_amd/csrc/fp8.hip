@@ -212,120 +212,80 @@ __device__ __forceinline__ typename M::Frag load32(const uint8_t* p) {
 
 // ---- the product of few rows -----------------------------------------------------------------
 // Bound by reading the items once: operands go straight from memory to registers, up to PF blocks
-// of a wave in flight.  A wave holds 16 NT items x 16 MT queries; the KS waves of a workgroup take every
-// KS-th block of the same rows and are summed through LDS, in order of the wave.
-template <typename T, int NT, int MT, int KS, int PF>
+// of a wave in flight.  A workgroup takes 16 items x 16 queries; its KS waves take every KS-th block of the
+// same rows and are summed through LDS, in order of the wave.  1 x 25,216 x 384 to f32: 4.1 us, of which the launch
+// is 2; 1 x 100,000 x 768: 15.5 us, 5.0 TB/s.
+template <typename T, int KS, int PF>
 __global__ __launch_bounds__(KS * 64) void product_few_kernel(ProductArgs a, int n_groups) {
-  typedef typename Mode<T>::Frag Frag;
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)(blockIdx.x % n_groups) * 16 * NT, m0 = (int64_t)(blockIdx.x / n_groups) * 16 * MT;
-  const uint8_t *xp[NT], *qp[MT];
-  const float *xs[NT], *qs[MT];
-  const bool whole = n0 + 16 * NT <= a.N;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t n = n0 + t * 16 + r;
-    xp[t] = a.x + (n < a.N ? n : a.N - 1) * a.ldx + g * 32;
-    const int64_t s = n0 + t * 16 + g * 4;
-    xs[t] = a.xs + (a.tile ? n0 / kBlock : s < a.N ? s : a.N - 1);
-  }
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int64_t m = m0 + t * 16 + r < a.M ? m0 + t * 16 + r : a.M - 1;
-    qp[t] = a.q + m * a.ldq + g * 32;
-    qs[t] = a.qs + m;
-  }
-  f32x4 acc[MT][NT] = {};
+  const int64_t n0 = (int64_t)(blockIdx.x % n_groups) * 16, m0 = (int64_t)(blockIdx.x / n_groups) * 16;
+  const bool whole = n0 + 16 <= a.N;
+  // rows past the end repeat the last one: their results are not stored
+  const int64_t nr = n0 + r < a.N ? n0 + r : a.N - 1, mr = m0 + r < a.M ? m0 + r : a.M - 1;
+  const int64_t n = n0 + g * 4, m = m0 + r;  // this lane's scores: items n .. n + 3 of query m
+  const uint8_t* xp = a.x + nr * a.ldx + g * 32;
+  const uint8_t* qp = a.q + mr * a.ldq + g * 32;
+  const float* xs = a.xs + (a.tile ? n0 / kBlock : n < a.N ? n : a.N - 1);
+  const float* qs = a.qs + mr;
+  f32x4 acc{0.f, 0.f, 0.f, 0.f};
   for (int b0 = wave; b0 < a.kb; b0 += KS * PF) {
-    u32x4 x[PF][NT][2], q[PF][MT][2];
-    f32x4 sx[PF][NT];
-    float sq[PF][MT];
+    u32x4 x[PF][2], q[PF][2];
+    f32x4 sx[PF];
+    float sq[PF];
 #pragma unroll
     for (int f = 0; f < PF; ++f) {
-      const int b = b0 + f * KS < a.kb ? b0 + f * KS : b0;  // (a block past the end counts 0 below)
+      const int b = b0 + f * KS < a.kb ? b0 + f * KS : b0;  // (a block past the end is not used below)
+      const u32x4* px = (const u32x4*)(xp + (int64_t)b * kBlock);
+      const u32x4* pq = (const u32x4*)(qp + (int64_t)b * kBlock);
+      const float* s = xs + b * a.ldxs;
+      x[f][0] = px[0];
+      x[f][1] = px[1];
+      q[f][0] = pq[0];
+      q[f][1] = pq[1];
+      sq[f] = qs[b * a.ldqs];
+      if (a.tile) {
+        sx[f] = f32x4{*s, *s, *s, *s};
+      } else if (whole) {
+        sx[f] = *(const f32x4u*)s;
+      } else {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const u32x4* p = (const u32x4*)(xp[t] + (int64_t)b * kBlock);
-        x[f][t][0] = p[0];
-        x[f][t][1] = p[1];
-      }
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const u32x4* p = (const u32x4*)(qp[t] + (int64_t)b * kBlock);
-        q[f][t][0] = p[0];
-        q[f][t][1] = p[1];
-        sq[f][t] = qs[t][b * a.ldqs];
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float* p = xs[t] + b * a.ldxs;
-        if (a.tile) {
-          sx[f][t] = f32x4{*p, *p, *p, *p};
-        } else if (whole) {
-          typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-          sx[f][t] = *(const f32x4u*)p;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) sx[f][t][j] = n0 + t * 16 + g * 4 + j < a.N ? p[j] : 0.f;
-        }
+        for (int j = 0; j < 4; ++j) sx[f][j] = n + j < a.N ? s[j] : 0.f;
       }
     }
 #pragma unroll
     for (int f = 0; f < PF; ++f) {
       if (b0 + f * KS >= a.kb) break;
-      Frag xf[NT];
+      const f32x4 p = Mode<T>::dot(Mode<T>::make(x[f][0], x[f][1]), Mode<T>::make(q[f][0], q[f][1]));
 #pragma unroll
-      for (int t = 0; t < NT; ++t) xf[t] = Mode<T>::make(x[f][t][0], x[f][t][1]);
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const Frag qf = Mode<T>::make(q[f][mt][0], q[f][mt][1]);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const f32x4 p = Mode<T>::dot(xf[t], qf);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[mt][t][j] = fmaf(sq[f][mt] * sx[f][t][j], p[j], acc[mt][t][j]);
-        }
-      }
+      for (int j = 0; j < 4; ++j) acc[j] = fmaf(sq[f] * sx[f][j], p[j], acc[j]);
     }
   }
   if constexpr (KS > 1) {
-    __shared__ f32x4 part[KS - 1][MT * NT][64];
-    if (wave > 0) {
-#pragma unroll
-      for (int i = 0; i < MT * NT; ++i) part[wave - 1][i][lane] = acc[i / NT][i % NT];
-    }
+    __shared__ f32x4 part[KS - 1][64];
+    if (wave > 0) part[wave - 1][lane] = acc;
     __syncthreads();
     if (wave > 0) return;
 #pragma unroll
-    for (int w = 0; w < KS - 1; ++w)
-#pragma unroll
-      for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += part[w][i][lane];
+    for (int w = 0; w < KS - 1; ++w) acc += part[w][lane];
   }
+  if (m >= a.M) return;
+  typedef T Out __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  T* p = (T*)a.out + m * a.ldo + n;
+  if (n + 4 <= a.N) {
+    *(Out*)p = Out{(T)acc[0], (T)acc[1], (T)acc[2], (T)acc[3]};
+  } else {
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int64_t m = m0 + mt * 16 + r;
-    if (m >= a.M) continue;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      typedef T Out __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-      const int64_t n = n0 + t * 16 + g * 4;
-      T* p = (T*)a.out + m * a.ldo + n;
-      if (n + 4 <= a.N) {
-        *(Out*)p = Out{(T)acc[mt][t][0], (T)acc[mt][t][1], (T)acc[mt][t][2], (T)acc[mt][t][3]};
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < a.N) p[j] = (T)acc[mt][t][j];
-      }
-    }
+    for (int j = 0; j < 4; ++j)
+      if (n + j < a.N) p[j] = (T)acc[j];
   }
 }
 
 // ---- the product of many rows: tiles staged through LDS ----------------------------------------
-// A workgroup of WN x WM waves computes 64 WN items x 16 MT WM queries; a wave 64 items x 16 MT
-// queries.  Both operands' blocks of 128 codes go to LDS by LDS-DMA, double buffered: the next
-// block's loads are in flight while this one's products run, one barrier to a block.  The block's
-// scales go along (4 bytes a row).
+// A group of WN x WM waves computes 64 WN items x 16 MT WM queries; a wave 64 items x 16 MT queries.  A
+// workgroup is KG such groups, which share out the blocks of the same rows and are summed at the end.  Both
+// operands' blocks of 128 codes go to LDS by LDS-DMA into D stages: the next block's loads are in flight
+// while this one's products run, one barrier to a block.  The block's scales go along (4 bytes a row).
 //
 // LDS rows are 128 bytes of 8 chunks; chunk c of row r sits at position c ^ f(r), with f such that the 8
 // rows that 8 neighbouring lanes read together have 8 different f: their 16-byte reads then fall
@@ -333,9 +293,9 @@ __global__ __launch_bounds__(KS * 64) void product_few_kernel(ProductArgs a, int
 //
 // Item rows are dealt to MFMA tiles so that a lane's results of V neighbouring tiles are 4 V
 // consecutive items: 16-byte stores, 64 bytes of a score row to each 4 lanes.
-template <typename T, int WN, int WM, int MT, int D>
+template <typename T, int WN, int WM, int MT, int D, int KG>
 struct TileShape {
-  static constexpr int kWaves = WN * WM, kThreads = kWaves * 64;
+  static constexpr int kWaves = WN * WM, kThreads = KG * kWaves * 64;  // waves of a group, threads of all
   static constexpr int V = 4 / (int)sizeof(T);
   static constexpr int TN = WN * 64, TM = WM * MT * 16;
   static constexpr int kX = TN * kBlock, kQ = TM * kBlock, kS = (TN + TM) * 4;
@@ -346,7 +306,8 @@ struct TileShape {
   static constexpr int kLoads = kXP + kQP + kSP;                       // loads of a wave and stage
   static_assert(TN % 64 == 0 && TM % 64 == 0, "whole pieces of 64 scales");
   static constexpr int kOut = TN * TM * (int)sizeof(T);                // the tile's scores, at the end
-  static constexpr int kLds = D * kStage > kOut ? D * kStage : kOut;
+  static constexpr int kJoin = (KG - 1) * TN * TM * 4;                 // the other groups' sums, at the end
+  static constexpr int kLds = KG * D * kStage > kOut + kJoin ? KG * D * kStage : kOut + kJoin;
   static_assert(D >= 2 && kLds <= 160 * 1024, "the stages fit the LDS");
   static_assert((D - 2) * kLoads < 64, "the wait counter holds the loads in flight");
   static __device__ __forceinline__ int fx(int n) { return (n & 3) | ((n >> (V == 1 ? 2 : 3)) & 1) << 2; }
@@ -357,9 +318,9 @@ __device__ __forceinline__ void lds_dma(uint32_t dst, uint32_t off, const void* 
   static_assert(BYTES == 4 || BYTES == 16, "dword and four-dword pieces");
   // (inline, so that the compiler's own waits leave these loads in flight)
   if constexpr (BYTES == 16)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(base) : "memory");
   else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(dst), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(dst)), "v"(off), "s"(base) : "memory");
 }
 template <typename P>
 __device__ __forceinline__ P* uniform(P* p) {
@@ -367,6 +328,12 @@ __device__ __forceinline__ P* uniform(P* p) {
   const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)v);
   const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(v >> 32));
   return (P*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// value K of a row of 16 lanes, in all of them
+template <int K>
+__device__ __forceinline__ float row_bcast(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + K, 0xf, 0xf, true));
 }
 
 // Workgroup -> tile: each XCD takes one contiguous run of tiles (its L2 then holds their rows), in
@@ -380,15 +347,16 @@ __device__ __forceinline__ void tile_of(int L, int total, int tiles_m, int tiles
   tn = j / rows;
 }
 
-template <typename T, bool TILE, int WN, int WM, int MT, int D>
-__global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
-  using S = TileShape<T, WN, WM, MT, D>;
+template <typename T, bool TILE, int WN, int WM, int MT, int D, int KG>
+__global__ __launch_bounds__(KG* WN* WM * 64, KG* WN* WM > 8 ? KG * WN * WM / 4 : 2) void product_tile_kernel(ProductArgs a, int tiles_m, int tiles_n) {
+  using S = TileShape<T, WN, WM, MT, D, KG>;
   constexpr int V = S::V;
   __shared__ __attribute__((aligned(1024))) char smem[S::kLds];
   int tm, tn;
   tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
   const int64_t n0 = (int64_t)tn * S::TN, m0 = (int64_t)tm * S::TM;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = all / S::kWaves, wave = all % S::kWaves;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wn = wave % WN, wm = wave / WN;
   const int nx = (int)(a.N - n0 < S::TN ? a.N - n0 : S::TN), nq = (int)(a.M - m0 < S::TM ? a.M - m0 : S::TM);
 
@@ -408,7 +376,7 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArg
   const uint8_t* qb = uniform(a.q + m0 * a.ldq);
   const float* xsb = uniform(a.xs + (TILE ? n0 / kBlock : n0));
   const float* qsb = uniform(a.qs + m0);
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem + group * D * S::kStage;
   auto stage = [&](int b, int buf) __attribute__((always_inline)) {
     const uint32_t at = lds0 + buf * S::kStage;
     const uint8_t* x = xb + (int64_t)b * kBlock;
@@ -441,17 +409,22 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArg
   qat = S::kX + (wm * MT * 16 + r) * kBlock + ((g ^ (r & 7)) << 4);
 
   f32x4 acc[MT][4] = {};
-  // D stages: while block b is computed, blocks b + 1 .. b + D - 1 are in flight.  (Past the last block
-  // the last one is loaded again, into a stage that nobody reads, so that the count stays the same.)
-  auto at_most = [&](int b) { return b < a.kb ? b : a.kb - 1; };
+  // Group `group` of KG takes blocks group, group + KG, ...; its step i is block i KG + group.  D stages a group:
+  // while a step is computed, the next D - 1 are in flight.
+  auto block = [&](int i) { return i * KG + group; };
 #pragma unroll
-  for (int i = 0; i < D - 1; ++i) stage(at_most(i), i);
+  for (int i = 0; i < D - 1; ++i)
+    if (block(i) < a.kb) stage(block(i), i);
   int cur = 0;
-  for (int b = 0; b < a.kb; ++b) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * S::kLoads) : "memory");
-    __syncthreads();  // block b is in for every wave, and the stage of block b - 1 is free
-    stage(at_most(b + D - 1), cur == 0 ? D - 1 : cur - 1);
-    const char* at = smem + cur * S::kStage;
+  for (int i0 = 0; i0 * KG < a.kb; ++i0) {
+    if (D > 2 && block(i0 + D - 2) < a.kb)
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 2) * S::kLoads) : "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();  // this step's block is in for every wave, and the stage of the step before is free
+    if (block(i0 + D - 1) < a.kb) stage(block(i0 + D - 1), cur == 0 ? D - 1 : cur - 1);
+    if (KG > 1 && block(i0) >= a.kb) break;  // (the last step, for the groups without a block in it)
+    const char* at = smem + group * D * S::kStage + cur * S::kStage;
     cur = cur + 1 == D ? 0 : cur + 1;
     const float* sc = (const float*)(at + S::kX + S::kQ);
     typedef typename Mode<T>::Frag Frag;
@@ -500,8 +473,23 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArg
     add(MT * 4 - 2);
     add(MT * 4 - 1);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
+  if constexpr (KG > 1) {
+    // the groups' sums, added in the groups' order
+    f32x4* part = (f32x4*)(smem + S::kOut) + wave * 64 + lane;
+    constexpr int kStep = S::kWaves * 64;
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < MT * 4; ++i) part[((group - 1) * MT * 4 + i) * kStep] = acc[i / 4][i % 4];
+    }
+    __syncthreads();
+    if (group == 0) {
+#pragma unroll
+      for (int w = 0; w < KG - 1; ++w)
+#pragma unroll
+        for (int i = 0; i < MT * 4; ++i) acc[i / 4][i % 4] += part[(w * MT * 4 + i) * kStep];
+    }
+  }
 
   // The results are turned around in the LDS (all reads of the stages are done), so that a store covers
   // 1 KiB of the tile's score rows, each row's part whole: full lines but for a row's two ends.
@@ -510,6 +498,7 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArg
   static_assert(kChunks <= 64, "a store covers whole rows");
   typedef T Out __attribute__((ext_vector_type(4 * V)));
   typedef T OutAt __attribute__((ext_vector_type(4 * V), aligned(sizeof(T))));
+  if (KG == 1 || group == 0) {
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     char* row = smem + (wm * MT * 16 + mt * 16 + r) * kRow;
@@ -521,15 +510,17 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArg
       *(Out*)(row + (((wn * 16 / V + u * 4 + g) ^ (r & kSwz)) << 4)) = v;
     }
   }
+  }
   __syncthreads();
   const int c = threadIdx.x & (kChunks - 1);
   const int64_t n = n0 + c * 4 * V;
   if (n >= a.N) return;
+  constexpr int kRows = S::kThreads / kChunks;  // rows of one store by all threads
 #pragma unroll
-  for (int i = 0; i < S::TM * kChunks / S::kThreads; ++i) {
-    const int row = i * (S::kThreads / kChunks) + threadIdx.x / kChunks;
+  for (int i = 0; i < (S::TM + kRows - 1) / kRows; ++i) {
+    const int row = i * kRows + threadIdx.x / kChunks;
     const int64_t m = m0 + row;
-    if (m >= a.M) break;
+    if (row >= S::TM || m >= a.M) break;
     const Out v = *(const Out*)(smem + row * kRow + ((c ^ (row & kSwz)) << 4));
     T* p = (T*)a.out + m * a.ldo + n;
     if (n + 4 * V <= a.N) {
@@ -542,6 +533,259 @@ __global__ __launch_bounds__(WN* WM * 64, 2) void product_tile_kernel(ProductArg
   }
 }
 
+// ---- 16-bit scores of many rows: one workgroup a CU, tile after tile --------------------------------
+// Tiles of 256 x 256, 8 waves of 64 items x 128 queries, two stages.  What the LDS has to deliver bounds it
+// (192 KB a block to the 8 waves, beside 64 KB that come in), then the matrix cores, then the scaling (4 or 8
+// FMA slots beside each product of 16 x 16 x 128).  Hence:
+//  - a block's last two query tiles are multiplied item tile by item tile, and as soon as an item tile is done
+//    its registers take the next block's: the burst of reads that opens a block runs beside products;
+//  - one barrier a block, before those last products: all reads of the block are done, the next block is in;
+//  - the loader runs ahead over the tiles' ends, and a tile's scores go out beside the next tile's blocks;
+//  - a product is scaled two products later.  The empty asm keeps the compiler from collecting the sums at the
+//    end of the block, which would hold all 32 products in registers.
+// 4,096 x 8,192 x 4,096: 126 us, 2.18 PFLOP/s (135 us with a workgroup to a tile; 3.2 PFLOP/s is what a large 8-bit
+// product without block scales reaches).  4,096 x 125,000 x 768, whose rows begin anywhere in a line: 664 us against
+// 743 with tiles of 128 and 722 with 128 bytes of a row to a store; from 124,928 items, whose rows begin at
+// lines, 128 bytes take 545 us and 512 take 615.
+template <typename T>
+using RunShape = TileShape<T, 4, 2, 8, 2, 1>;  // 256 x 256
+constexpr int kCus = 256;
+
+template <typename T, bool TILE, bool LINES>
+__global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int tiles_m, int tiles_n) {
+  using S = RunShape<T>;
+  constexpr int V = S::V, WN = 4, MT = 8;
+  static_assert(V == 2 && S::kThreads == 512, "16-bit scores");
+  constexpr int kOwn = LINES ? 16 * 64 * 2 : 0;  // a wave's 16 x 64 scores
+  static_assert(2 * S::kStage + S::kWaves * kOwn <= 160 * 1024, "the stages and the waves' turning places fit the LDS");
+  __shared__ __attribute__((aligned(1024))) char smem[2 * S::kStage + S::kWaves * kOwn];
+  const int total = tiles_m * tiles_n;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wn = wave % WN, wm = wave / WN;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+
+  // the loader: the next block of the next tile to go to the LDS
+  int d_tile = blockIdx.x, d_b = 0;
+  uint32_t xoff[S::kXP], qoff[S::kQP], soff[S::kSP];
+  const uint8_t *xb, *qb;
+  const float *xsb, *qsb;
+  auto aim = [&]() __attribute__((always_inline)) {
+    int tm, tn;
+    tile_of(d_tile, total, tiles_m, tiles_n, tm, tn);
+    const int64_t n0 = (int64_t)tn * S::TN, m0 = (int64_t)tm * S::TM;
+    const int nx = (int)(a.N - n0 < S::TN ? a.N - n0 : S::TN), nq = (int)(a.M - m0 < S::TM ? a.M - m0 : S::TM);
+#pragma unroll
+    for (int p = 0; p < S::kXP; ++p) {
+      const int row = (wave * S::kXP + p) * 8 + (lane >> 3);
+      xoff[p] = (uint32_t)(row < nx ? row : nx - 1) * (uint32_t)a.ldx + (((lane & 7) ^ S::fx(row)) << 4);
+    }
+#pragma unroll
+    for (int p = 0; p < S::kQP; ++p) {
+      const int row = (wave * S::kQP + p) * 8 + (lane >> 3);
+      qoff[p] = (uint32_t)(row < nq ? row : nq - 1) * (uint32_t)a.ldq + (((lane & 7) ^ (row & 7)) << 4);
+    }
+#pragma unroll
+    for (int j = 0; j < S::kSP; ++j) {
+      const int i = (j * S::kWaves + wave) % ((S::TN + S::TM) / 64);
+      const int row = (i < S::TN / 64 ? i : i - S::TN / 64) * 64 + lane, n = i < S::TN / 64 ? nx : nq;
+      const int c = row < n ? row : n - 1;
+      soff[j] = (uint32_t)(TILE && i < S::TN / 64 ? c / kBlock : c) * 4;
+    }
+    xb = a.x + n0 * a.ldx;
+    qb = a.q + m0 * a.ldq;
+    xsb = a.xs + (TILE ? n0 / kBlock : n0);
+    qsb = a.qs + m0;
+  };
+  auto load_next = [&](int buf) __attribute__((always_inline)) {
+    if (d_tile >= total) return;
+    const uint32_t at = lds0 + buf * S::kStage;
+    const uint8_t* x = uniform(xb + (int64_t)d_b * kBlock);
+    const uint8_t* q = uniform(qb + (int64_t)d_b * kBlock);
+#pragma unroll
+    for (int p = 0; p < S::kXP; ++p) lds_dma<16>(at + (wave * S::kXP + p) * 1024, xoff[p], x);
+#pragma unroll
+    for (int p = 0; p < S::kQP; ++p) lds_dma<16>(at + S::kX + (wave * S::kQP + p) * 1024, qoff[p], q);
+#pragma unroll
+    for (int j = 0; j < S::kSP; ++j) {
+      const int i = (j * S::kWaves + wave) % ((S::TN + S::TM) / 64);
+      const float* base = i < S::TN / 64 ? xsb + d_b * a.ldxs : qsb + d_b * a.ldqs;
+      lds_dma<4>(at + S::kX + S::kQ + i * 256, soff[j], uniform(base));
+    }
+    if (++d_b == a.kb) {
+      d_b = 0;
+      d_tile += gridDim.x;
+      if (d_tile < total) aim();
+    }
+  };
+
+  auto x_tile = [](int t) { return ((t / V) * 16 * V + (t % V) * 4) * kBlock; };
+  const int xrow = wn * 64 + (r >> 2) * 4 * V + (r & 3);
+  const uint32_t xat = xrow * kBlock + ((g ^ S::fx(xrow)) << 4);
+  const uint32_t qat = S::kX + (wm * MT * 16 + r) * kBlock + ((g ^ (r & 7)) << 4);
+  auto load_x = [&](const char* at, int t) __attribute__((always_inline)) {
+    return Narrow::make(*(const u32x4*)(at + xat + x_tile(t)), *(const u32x4*)(at + (xat ^ 64) + x_tile(t)));
+  };
+  auto load_q = [&](const char* at, int mt) __attribute__((always_inline)) {
+    return Narrow::make(*(const u32x4*)(at + qat + mt * 16 * kBlock), *(const u32x4*)(at + (qat ^ 64) + mt * 16 * kBlock));
+  };
+  constexpr int kTail = 2, LAG = 2;
+
+  aim();
+  load_next(0);
+  load_next(1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  i32x8 x[4], qr[2];
+  qr[0] = load_q(smem, 0);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) x[t] = load_x(smem, t);
+  int cur = 0;
+  for (int tile = blockIdx.x; tile < total; tile += gridDim.x) {
+    f32x4 acc[MT][4] = {};
+    for (int b = 0; b < a.kb; ++b) {
+      const char* at = smem + cur * S::kStage;
+      const char* nat = smem + (cur ^ 1) * S::kStage;
+      const float* sc = (const float*)(at + S::kX + S::kQ);
+      i32x8 q[MT];
+      float sq[MT], sxv;
+      f32x4 p[LAG + 1];
+      sxv = TILE ? sc[wn * 64] : sc[wn * 64 + (r / (4 * V)) * 16 * V + g * 4 * V + ((r >> 2) % V) * 4 + (r & 3)];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sq[mt] = sc[S::TN + wm * MT * 16 + mt * 16 + r];
+      qr[1] = load_q(at, 1);
+      q[0] = qr[0];
+      if constexpr (TILE) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) sq[mt] *= sxv;
+      }
+      auto qi = [](int i) { return i < (MT - kTail) * 4 ? i / 4 : MT - kTail + (i - (MT - kTail) * 4) % kTail; };
+      auto xi = [](int i) { return i < (MT - kTail) * 4 ? i % 4 : (i - (MT - kTail) * 4) / kTail; };
+      auto add = [&](int i) __attribute__((always_inline)) {
+        const int mt = qi(i), t = xi(i);
+        const float s = sq[mt];
+        f32x4 f = {s, s, s, s};
+        if constexpr (!TILE) {
+          if (t == 0) f = f32x4{row_bcast<0>(sxv) * s, row_bcast<1>(sxv) * s, row_bcast<2>(sxv) * s, row_bcast<3>(sxv) * s};
+          if (t == 1) f = f32x4{row_bcast<4>(sxv) * s, row_bcast<5>(sxv) * s, row_bcast<6>(sxv) * s, row_bcast<7>(sxv) * s};
+          if (t == 2) f = f32x4{row_bcast<8>(sxv) * s, row_bcast<9>(sxv) * s, row_bcast<10>(sxv) * s, row_bcast<11>(sxv) * s};
+          if (t == 3) f = f32x4{row_bcast<12>(sxv) * s, row_bcast<13>(sxv) * s, row_bcast<14>(sxv) * s, row_bcast<15>(sxv) * s};
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[mt][t][j] = fmaf(f[j], p[i % (LAG + 1)][j], acc[mt][t][j]);
+        asm volatile("" : "+v"(acc[mt][t]));
+      };
+#pragma unroll
+      for (int i = 0; i < MT * 4; ++i) {
+        const int mt = qi(i), t = xi(i);
+        if (i == (MT - kTail) * 4) {
+          q[MT - 1] = qr[(MT - 1) & 1];
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        p[i % (LAG + 1)] = Narrow::dot(x[t], q[mt]);
+        if (i < (MT - kTail) * 4) {
+          if (t == 0 && mt + 1 < MT) q[mt + 1] = qr[(mt + 1) & 1];
+          if (t == 1 && mt + 2 < MT) qr[mt & 1] = load_q(at, mt + 2);
+        } else if ((i - (MT - kTail) * 4) % kTail == kTail - 1) {
+          x[t] = load_x(nat, t);  // (after the last block of all: an old stage's, unused)
+          if (t == 0) qr[0] = load_q(nat, 0);
+        }
+        if (i >= LAG) add(i - LAG);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = MT * 4 - LAG; i < MT * 4; ++i) add(i);
+      if (LINES || b + 1 < a.kb) load_next(cur);
+      cur ^= 1;
+    }
+
+    int tm, tn;
+    tile_of(tile, total, tiles_m, tiles_n, tm, tn);
+    typedef T Out __attribute__((ext_vector_type(8)));
+    typedef T OutAt __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+    if constexpr (LINES) {
+      // A wave turns 16 of its rows at a time around in a place of its own: a store covers 128 bytes of 8 rows, a
+      // whole line of each, while the next tile's two first blocks come in.
+      const int64_t n0 = (int64_t)tn * S::TN + wn * 64, m0 = (int64_t)tm * S::TM + wm * MT * 16;
+      char* own = smem + 2 * S::kStage + wave * kOwn;
+      const int64_t n = n0 + (lane & 7) * 8;
+      T* out = (T*)a.out + (m0 + (lane >> 3)) * a.ldo + n;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          Out v;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = (T)acc[mt][u * 2 + (j >> 2)][j & 3];
+          *(Out*)(own + r * 128 + (((u * 4 + g) ^ (r & 7)) << 4)) = v;
+        }
+        __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses are in order; this keeps the compiler's so)
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int row = h * 8 + (lane >> 3);
+          const Out v = *(const Out*)(own + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
+          if (m0 + mt * 16 + row < a.M) {
+            T* p = out + (int64_t)(mt * 16 + h * 8) * a.ldo;
+            if (n + 8 <= a.N) {
+              __builtin_nontemporal_store(OutAt(v), (OutAt*)p);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) p[j] = v[j];
+            }
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+      }
+    } else {
+      // Rows that do not begin at a line: 128 bytes of a row are parts of two lines, and parts of lines written past
+      // the L2 cost twice.  The scores are turned around in the last block's stage, half the tile's queries at a
+      // time, so that a store covers 512 bytes of a row; the stage is loaded again after that.
+      constexpr int kRow = S::TN * 2, kHalf = S::TM / 2;
+      static_assert(kHalf * kRow <= S::kStage && kRow == 512, "half a tile's scores fit a stage");
+      char* turn = smem + (cur ^ 1) * S::kStage;
+      const int c = threadIdx.x & 31;
+      const int64_t n = (int64_t)tn * S::TN + c * 8;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < MT / 2; ++i) {
+          char* row = turn + (wm * (kHalf / 2) + i * 16 + r) * kRow;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            Out v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = (T)acc[h * (MT / 2) + i][u * 2 + (j >> 2)][j & 3];
+            *(Out*)(row + (((wn * 8 + u * 4 + g) ^ r) << 4)) = v;
+          }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kHalf / 16; ++i) {
+          const int row = i * 16 + (threadIdx.x >> 5);
+          const int64_t m = (int64_t)tm * S::TM + (row / (kHalf / 2)) * (S::TM / 2) + h * (kHalf / 2) + row % (kHalf / 2);
+          const Out v = *(const Out*)(turn + row * kRow + ((c ^ (row & 15)) << 4));
+          if (m < a.M) {
+            T* p = (T*)a.out + m * a.ldo + n;
+            if (n + 8 <= a.N) {
+              __builtin_nontemporal_store(OutAt(v), (OutAt*)p);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n + j < a.N) p[j] = v[j];
+            }
+          }
+        }
+        __syncthreads();
+      }
+      load_next(cur ^ 1);
+    }
+  }
+}
+
 // ---- which kernel ---------------------------------------------------------------------------
 int too_many() { return abi_fail(BB_E_ARG, "bb_scores_fp8: too many scores for one call"); }
 
@@ -549,37 +793,67 @@ template <typename T, int KS, int PF>
 int launch_few(const ProductArgs& a, void* stream) {
   const int64_t n_groups = (a.N + 15) / 16, total = n_groups * ((a.M + 15) / 16);
   if (total > (int64_t)(0xFFFFFFFFu / (KS * 64))) return too_many();
-  return abi_launch("bb_scores_fp8", product_few_kernel<T, 1, 1, KS, PF>, dim3((uint32_t)total), dim3(KS * 64), 0,
+  return abi_launch("bb_scores_fp8", product_few_kernel<T, KS, PF>, dim3((uint32_t)total), dim3(KS * 64), 0,
                     (hipStream_t)stream, a, (int)n_groups);
 }
 
-template <typename T, int WN, int WM, int MT, int D>
+template <typename T, int WN, int WM, int MT, int D, int KG>
 int launch_tile(const ProductArgs& a, void* stream) {
-  using S = TileShape<T, WN, WM, MT, D>;
+  using S = TileShape<T, WN, WM, MT, D, KG>;
   const int64_t tiles_m = (a.M + S::TM - 1) / S::TM, tiles_n = (a.N + S::TN - 1) / S::TN;
   if (tiles_m * tiles_n > (int64_t)(0xFFFFFFFFu / S::kThreads)) return too_many();
-  return abi_launch("bb_scores_fp8", a.tile ? product_tile_kernel<T, true, WN, WM, MT, D> : product_tile_kernel<T, false, WN, WM, MT, D>,
+  return abi_launch("bb_scores_fp8",
+                    a.tile ? product_tile_kernel<T, true, WN, WM, MT, D, KG> : product_tile_kernel<T, false, WN, WM, MT, D, KG>,
                     dim3((uint32_t)(tiles_m * tiles_n)), dim3(S::kThreads), 0, (hipStream_t)stream, a, (int)tiles_m,
+                    (int)tiles_n);
+}
+
+template <typename T>
+int launch_run(const ProductArgs& a, void* stream) {
+  using S = RunShape<T>;
+  const int64_t tiles_m = (a.M + S::TM - 1) / S::TM, tiles_n = (a.N + S::TN - 1) / S::TN, total = tiles_m * tiles_n;
+  if (total > 0x7FFFFFFF / 2) return too_many();
+  const bool lines = (uintptr_t)a.out % 128 == 0 && a.ldo % 64 == 0;
+  return abi_launch("bb_scores_fp8", lines ? (a.tile ? product_run_kernel<T, true, true> : product_run_kernel<T, false, true>)
+                                           : (a.tile ? product_run_kernel<T, true, false> : product_run_kernel<T, false, false>),
+                    dim3((uint32_t)(total < kCus ? total : kCus)), dim3(S::kThreads), 0, (hipStream_t)stream, a, (int)tiles_m,
                     (int)tiles_n);
 }
 
 inline int64_t tiles(const ProductArgs& a, int t) { return ((a.M + t - 1) / t) * ((a.N + t - 1) / t); }
 inline int64_t up(int64_t x, int64_t by) { return (x + by - 1) / by; }
 
+// Times below: M x N x K on one MI355X, kernel alone, "against" = the other choice.
 template <typename T>
 int launch_product(const ProductArgs& a, void* stream) {
-  // The tiles' source offsets are 32-bit within 256 rows.
+  // The tiles' source offsets are 32-bit within 256 rows; rows further apart are read by their 64-bit addresses.
   const bool far = a.ldx >= (1 << 24) || a.ldq >= (1 << 24);
-  if (a.M <= 16 || far) {
-    // one block a wave while it is short (3 blocks, 25,216 items, 1 query: 4.1 us against 8.3 with 8 waves and
-    // 6.2 with one), longer rows split over more waves (32 blocks, 8,192 items, 16 queries: 12.1 us against 13.3)
-    return a.kb == 1 ? launch_few<T, 1, 1>(a, stream) : a.kb <= 8 ? launch_few<T, 4, 1>(a, stream) : launch_few<T, 8, 2>(a, stream);
+  const bool split = tiles(a, 64) <= kCus && a.kb >= 8;  // fewer 64 x 64 tiles than CUs, and long rows: split the rows
+  bool few = a.M <= 16;
+  // 9 to 16 rows waste less of a tile: against a long list of items it reads them in larger pieces (16 x 50,000 x 1,024
+  // 10.9 us against 15.2; 1 x 100,000 x 768 19.1 against 15.5), and against 6,144 to 16,384 items long rows are
+  // better split in it (16 x 8,192 x 4,096 10.1 us against 12.0; 16 x 4,096 x 4,096 9.7 against 7.1)
+  if (a.M > 8 && a.M <= 16) few = !(a.N >= 32768 || (split && tiles(a, 64) >= 96));
+  // few scores and long rows: 20 x 300 x 8,192 9.8 us against 24.9; 64 x 2,048 x 4,096 (512) 10.4 against 8.8
+  if (a.M > 16 && split && tiles(a, 16) <= 256) few = true;
+  if (few || far) {
+    if (a.kb == 1) return launch_few<T, 1, 1>(a, stream);
+    // one block a wave: 1 x 25,216 x 384 4.1 us against 8.3 with 8 waves of two
+    if (a.kb <= 8) return launch_few<T, 4, 1>(a, stream);
+    // two blocks of a wave in flight need the registers of other workgroups: 4 x 20,000 x 2,048 10.1 us with one
+    // against 13.7, 16 x 4,096 x 4,096 8.3 against 7.1
+    return a.N > 16384 ? launch_few<T, 8, 1>(a, stream) : launch_few<T, 8, 2>(a, stream);
   }
-  if (tiles(a, 128) < 200) return launch_tile<T, 1, 4, 1, 3>(a, stream);
+  // 64 x 8,192 x 4,096 10.9 us against 13.0 unsplit, 128 x 2,048 x 8,192 17.4 against 23.2
+  if (split) return launch_tile<T, 1, 4, 1, 2, 4>(a, stream);
+  // 40 x 100,000 x 384 f32 14.6 us against 18.6 with tiles of 128; 128 x 25,216 x 384 f32 (197 tiles) 8.8 against 8.2
+  if (a.M <= 64 || tiles(a, 128) < 192) return launch_tile<T, 1, 4, 1, 2, 1>(a, stream);
   if constexpr (sizeof(T) == 2) {
-    if (21 * up(tiles(a, 256), 256) <= 11 * up(tiles(a, 128), 512)) return launch_tile<T, 4, 2, 8, 2>(a, stream);
+    // rounds over the chip: one 256 x 256 tile a CU takes 1.8 times what two 128 x 128 tiles a CU do (4,096 x 8,192 x 4,096:
+    // 2 rounds 126 us against 4 rounds 145; 1,024 x 8,192 x 8,192: half a round 98 us against one 74)
+    if (9 * up(tiles(a, 256), kCus) <= 5 * up(tiles(a, 128), 2 * kCus)) return launch_run<T>(a, stream);
   }
-  return launch_tile<T, 2, 2, 4, 2>(a, stream);
+  return launch_tile<T, 2, 2, 4, 2, 1>(a, stream);
 }
 
 int check_rows(const bb_fp8_rows* r, const std::string& what) {
