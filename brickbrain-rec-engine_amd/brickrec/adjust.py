@@ -3,7 +3,7 @@
 the ``stream`` given, no synchronisation.  No gradient flows through the call."""
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional, Union
 
 import torch
@@ -23,36 +23,41 @@ def mask_words(mask: torch.Tensor) -> torch.Tensor:
     return (pad.to(torch.int64) << bit).sum(-1).to(torch.int32)
 
 
-_IDS = (torch.int32, torch.int64)
-_F32 = (torch.float32,)
-_WORDS = (torch.int32, torch.uint32)
+# bb_adjust packed into bytes (a third of the time of a ctypes structure); its fields in order
+_PACK = struct.Struct("@PPqqqqiiPqqPPPPfffPPqqPq").pack
+_IDS = {torch.int32: 0, torch.int64: 1}
+_F32 = {torch.float32: 0}
+_WORDS = {torch.int32: 0, torch.uint32: 0}
 
 
 def _list(t, name, dtypes, B, dev):
     """A list for each row [B, m], or one for all [m] -> (tensor, entries, elements between rows)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != dev:
         raise TypeError(f"{name} is a tensor of {' or '.join(str(d) for d in dtypes)} on cuda:{dev}")
-    if t.dim() == 1:
-        return t.contiguous(), t.shape[0], 0
-    if t.dim() != 2 or t.shape[0] != B:
-        raise ValueError(f"{name} is [{B}, m] or [m]: got {tuple(t.shape)}")
-    if t.is_contiguous():
-        m = t.shape[1]
-        return t, m, m or 1
-    if t.stride(0) == 0 and t.stride(1) == 1:  # one list expanded over the rows
-        return t, t.shape[1], 0
-    t = _rows_of(t)
-    return t, t.shape[1], _ld(t)
+    shape = t.shape
+    if len(shape) == 2 and shape[0] == B:
+        m = shape[1]
+        if t.is_contiguous():
+            return t, m, m or 1
+        if t.stride(0) == 0 and t.stride(1) == 1:  # one list expanded over the rows
+            return t, m, 0
+        t = _rows_of(t)
+        return t, m, _ld(t)
+    if len(shape) != 1:
+        raise ValueError(f"{name} is [{B}, m] or [m]: got {tuple(shape)}")
+    return t.contiguous(), shape[0], 0
 
 
 def _per_row(v: Number, name, B, dev):
-    """A value for all rows, or a tensor of one for each -> (pointer or None, value, tensor)."""
-    if isinstance(v, torch.Tensor):
-        if v.dtype is not torch.float32 or v.get_device() != dev or v.dim() != 1 or v.shape[0] != B:
-            raise TypeError(f"{name} is a number or a float32 tensor [{B}] on cuda:{dev}")
-        v = v.contiguous()
-        return v.data_ptr(), 0.0, v
-    return None, float(v), None
+    """A value for all rows, or a tensor of one for each -> (pointer or 0, value, tensor)."""
+    if not isinstance(v, torch.Tensor):
+        return 0, float(v), None
+    if v.dtype is not torch.float32 or v.get_device() != dev or tuple(v.shape) != (B,):
+        raise TypeError(f"{name} is a number or a float32 tensor [{B}] on cuda:{dev}")
+    if v.requires_grad:
+        _refuse_grad(v)
+    v = v.contiguous()
+    return v.data_ptr(), 0.0, v
 
 
 def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
@@ -80,8 +85,8 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         with _On(stream, scores.device, (scores, seen, seen_len, repetition, presence, frequency, bias_ids, bias, mask, out)):
             return adjust_scores(scores, seen=seen, seen_len=seen_len, repetition=repetition, presence=presence,
                                  frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, out=out)
-    if torch.is_grad_enabled():
-        _refuse_grad(*(t for t in (scores, repetition, presence, frequency, bias) if isinstance(t, torch.Tensor)))
+    if scores.requires_grad:
+        _refuse_grad(scores)
     B, n = scores.shape
     dev = scores.get_device()
     scores = _rows_of(scores)
@@ -92,12 +97,12 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         _check_out(out, (B, n), scores.dtype, scores.device)
         ld = _ld(out)
     # every tensor that the launch reads has a name here until it is out
-    seen_p = seen_len_p = rep_p = pre_p = fre_p = bias_ids_p = bias_p = mask_p = None
+    seen_p = seen_len_p = rep_p = pre_p = fre_p = bias_ids_p = bias_p = mask_p = 0
     n_seen = ld_seen = n_bias = ld_bias = ld_mask = ids64 = 0
     rep, pre, fre = 1.0, 0.0, 0.0
     if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
         raise ValueError(f"repetition is above 0: got {repetition}")
-    if seen is not None and bias_ids is not None and {seen.dtype, bias_ids.dtype} == set(_IDS):
+    if seen is not None and bias_ids is not None and seen.dtype is not bias_ids.dtype and {seen.dtype, bias_ids.dtype} == _IDS.keys():
         seen, bias_ids = seen.to(torch.int64), bias_ids.to(torch.int64)  # (the lists of one call have ids of one size)
     if seen is not None:
         seen, n_seen, ld_seen = _list(seen, "seen", _IDS, B, dev)
@@ -117,8 +122,10 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     if bias_ids is not None:
         bias_ids, n_bias, ld_bias = _list(bias_ids, "bias_ids", _IDS, B, dev)
         bias, m, ld_v = _list(bias, "bias", _F32, B, dev)
-        if bias.dim() != bias_ids.dim() or m != n_bias:
+        if m != n_bias or bias.dim() != bias_ids.dim():
             raise ValueError(f"bias is as bias_ids: got {tuple(bias.shape)} and {tuple(bias_ids.shape)}")
+        if bias.requires_grad:
+            _refuse_grad(bias)
         if ld_v != ld_bias:  # (the two lists share one distance between rows)
             bias_ids, bias = bias_ids.contiguous(), bias.contiguous()
             ld_bias = _ld(bias_ids)
@@ -133,9 +140,10 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         if w != (n + 31) // 32:
             raise ValueError(f"the mask of {n} scores has {(n + 31) // 32} words: got {w}")
         mask_p = mask.data_ptr()
-    a = L.bb_adjust(scores.data_ptr(), out.data_ptr(), B, n, _ld(scores), ld, _CODE[scores.dtype], ids64, seen_p, n_seen,
-                    ld_seen, seen_len_p, rep_p, pre_p, fre_p, rep, pre, fre, bias_ids_p, bias_p, n_bias, ld_bias, mask_p, ld_mask)
-    rc = L.load().bb_adjust_scores(dev, C.byref(a), _raw_stream(dev))
+    rc = L.load().bb_adjust_scores(
+        dev, _PACK(scores.data_ptr(), out.data_ptr(), B, n, _ld(scores), ld, _CODE[scores.dtype], ids64, seen_p, n_seen, ld_seen,
+                   seen_len_p, rep_p, pre_p, fre_p, rep, pre, fre, bias_ids_p, bias_p, n_bias, ld_bias, mask_p, ld_mask),
+        _raw_stream(dev))
     if rc:
         L.check(rc, "bb_adjust_scores")
     return out

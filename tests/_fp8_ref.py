@@ -43,8 +43,9 @@ def scores_bound(q, x, dtype):
     come from the 8-bit matrix instruction, which first cuts each product of a group of 8 at 2^-13 of
     the group's largest: 8 cuts lose at most 8 * 2^-13 = 2^-10 of that product, so at most 2^-10 of the sum
     of magnitudes over all groups."""
-    y = q @ x.t()
-    mag = q.abs() @ x.abs().t()
+    xt = x.t().contiguous()
+    y = q @ xt
+    mag = q.abs() @ xt.abs()
     kb = q.shape[1] // BLOCK
     cut = 0.0 if dtype == torch.float32 else 2.0 ** -10
     tol = (cut + BLOCK * 2.0 ** -23 + (kb + 18) * 2.0 ** -24) * mag

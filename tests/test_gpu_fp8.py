@@ -32,11 +32,13 @@ def quantized(br, n, d, tile=False, seed=0):
     return br.quantize_rows(make(n, d, seed=seed).to(DEV), tile=tile)
 
 
-def check_scores(q, x, got):
-    y, tol = R.scores_bound(R.values(q.codes.cpu(), q.scales.cpu(), q.tile), R.values(x.codes.cpu(), x.scales.cpu(), x.tile),
-                            got.dtype)
-    off = (got.double().cpu() - y).abs()
-    assert bool((off <= tol).all()), float((off / tol).max())
+def check_scores(q, x, got, dev="cpu"):
+    y, tol = R.scores_bound(*(R.values(r.codes.to(dev), r.scales.to(dev), r.tile) for r in (q, x)), got.dtype)
+    got, most = got.double().to(dev), torch.finfo(got.dtype).max
+    off = (got - y).abs()
+    # a sum that the bound lets reach the type's largest value (f16: 65504) rounds to the infinity of its sign
+    past = torch.isinf(got) & (y.abs() + tol >= most) & (torch.sign(got) == torch.sign(y))
+    assert bool(((off <= tol) | past).all()), float((off / tol)[~past].max())
 
 
 # ---- quantising -----------------------------------------------------------------------------
@@ -113,7 +115,21 @@ SIZES = [(1, 1, 1), (1, 64, 128), (1, 25216, 384), (2, 65, 129), (15, 257, 640),
 @pytest.mark.parametrize("m, n, k", SIZES)
 def test_scores(br, m, n, k, dtype, tile):
     q, x = quantized(br, m, k, seed=1), quantized(br, n, k, tile, seed=2)
-    check_scores(q, x, br.scores_fp8(q, x, dtype=dtype))
+    out = torch.full((m, n), float("nan"), dtype=dtype, device=DEV)
+    check_scores(q, x, br.scores_fp8(q, x, out=out))
+
+
+# enough tiles that a workgroup takes several, one after the other: rows of one block and more, edges inside the tiles,
+# score rows that begin at lines (ld) and anywhere
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k, ld", [(2040, 8190, 100, 8190), (2040, 8190, 300, 8192), (4090, 8100, 384, 8128), (4096, 8001, 130, 8001),
+                                         (1800, 20000, 200, 20000), (70, 60000, 128, 60000)])
+def test_scores_of_many_rows(br, m, n, k, ld, dtype, tile):
+    q, x = quantized(br, m, k, seed=1), quantized(br, n, k, tile, seed=2)
+    buf = torch.full((m, ld), float("nan"), dtype=dtype, device=DEV)
+    check_scores(q, x, br.scores_fp8(q, x, out=buf[:, :n]), DEV)
+    assert bool(torch.isnan(buf[:, n:]).all())
 
 
 @pytest.mark.parametrize("m, n, k", [(1, 70, 128), (20, 130, 300), (300, 270, 256)])
@@ -149,7 +165,13 @@ def test_rows_further_apart_than_32_bits(br):
     q = quantized(br, 5, 200, seed=5)
     assert torch.equal(br.scores_fp8(q, out), br.scores_fp8(q, near))
     assert torch.equal(br.scores_fp8(out, q), br.scores_fp8(near, q))
-    del far, out, store
+    # 20 rows 2^24 bytes apart: past what the tiles address, so read as a few rows are
+    wide = torch.as_strided(store, (20, 256), (1 << 24, 1)).view(torch.float8_e4m3fn)
+    rows = quantized(br, 20, 200, seed=6)
+    wide.copy_(rows.codes)
+    assert torch.equal(br.scores_fp8(br.Fp8Rows(wide, rows.scales, 200), rows, dtype=torch.bfloat16),
+                       br.scores_fp8(rows.part(0, 20), rows, dtype=torch.bfloat16))
+    del far, out, wide, store
     buf = torch.empty(2 * ld + 1024, dtype=torch.float16, device=DEV)
     y = torch.as_strided(buf, (3, 5), (ld, 1))
     br.scores_fp8(near, q, out=y)
