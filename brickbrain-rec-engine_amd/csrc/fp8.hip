@@ -539,9 +539,10 @@ __global__ __launch_bounds__(KG* WN* WM * 64, KG* WN* WM > 8 ? KG * WN * WM / 4 
 // FMA slots beside each product of 16 x 16 x 128).  Hence:
 //  - a block's last two query tiles are multiplied item tile by item tile, and as soon as an item tile is done
 //    its registers take the next block's: the burst of reads that opens a block runs beside products;
-//  - one barrier a block, before those last products: all reads of the block are done, the next block is in;
+//  - one barrier a block, before those last products: all reads of the block are done, the next block is in, and
+//    the loads of the one after it go out between them;
 //  - the loader runs ahead over the tiles' ends, and a tile's scores go out beside the next tile's blocks;
-//  - a product is scaled two products later.  The empty asm keeps the compiler from collecting the sums at the
+//  - a product is scaled three products later.  The empty asm keeps the compiler from collecting the sums at the
 //    end of the block, which would hold all 32 products in registers.
 // 4,096 x 8,192 x 4,096: 126 us, 2.18 PFLOP/s (135 us with a workgroup to a tile; 3.2 PFLOP/s is what a large 8-bit
 // product without block scales reaches).  4,096 x 125,000 x 768, whose rows begin anywhere in a line: 664 us against
@@ -596,26 +597,32 @@ __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int 
     xsb = a.xs + (TILE ? n0 / kBlock : n0);
     qsb = a.qs + m0;
   };
-  auto load_next = [&](int buf) __attribute__((always_inline)) {
-    if (d_tile >= total) return;
+  // load i of the S::kLoads that bring the loader's block into stage `buf`
+  auto load = [&](int i, int buf) __attribute__((always_inline)) {
     const uint32_t at = lds0 + buf * S::kStage;
-    const uint8_t* x = uniform(xb + (int64_t)d_b * kBlock);
-    const uint8_t* q = uniform(qb + (int64_t)d_b * kBlock);
-#pragma unroll
-    for (int p = 0; p < S::kXP; ++p) lds_dma<16>(at + (wave * S::kXP + p) * 1024, xoff[p], x);
-#pragma unroll
-    for (int p = 0; p < S::kQP; ++p) lds_dma<16>(at + S::kX + (wave * S::kQP + p) * 1024, qoff[p], q);
-#pragma unroll
-    for (int j = 0; j < S::kSP; ++j) {
-      const int i = (j * S::kWaves + wave) % ((S::TN + S::TM) / 64);
-      const float* base = i < S::TN / 64 ? xsb + d_b * a.ldxs : qsb + d_b * a.ldqs;
-      lds_dma<4>(at + S::kX + S::kQ + i * 256, soff[j], uniform(base));
+    if (i < S::kXP) {
+      lds_dma<16>(at + (wave * S::kXP + i) * 1024, xoff[i], uniform(xb + (int64_t)d_b * kBlock));
+    } else if (i < S::kXP + S::kQP) {
+      i -= S::kXP;
+      lds_dma<16>(at + S::kX + (wave * S::kQP + i) * 1024, qoff[i], uniform(qb + (int64_t)d_b * kBlock));
+    } else {
+      const int j = i - S::kXP - S::kQP, piece = (j * S::kWaves + wave) % ((S::TN + S::TM) / 64);
+      const float* base = piece < S::TN / 64 ? xsb + d_b * a.ldxs : qsb + d_b * a.ldqs;
+      lds_dma<4>(at + S::kX + S::kQ + piece * 256, soff[j], uniform(base));
     }
+  };
+  auto loaded = [&]() __attribute__((always_inline)) {
     if (++d_b == a.kb) {
       d_b = 0;
       d_tile += gridDim.x;
       if (d_tile < total) aim();
     }
+  };
+  auto load_next = [&](int buf) __attribute__((always_inline)) {
+    if (d_tile >= total) return;
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) load(i, buf);
+    loaded();
   };
 
   auto x_tile = [](int t) { return ((t / V) * 16 * V + (t % V) * 4) * kBlock; };
@@ -628,7 +635,7 @@ __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int 
   auto load_q = [&](const char* at, int mt) __attribute__((always_inline)) {
     return Narrow::make(*(const u32x4*)(at + qat + mt * 16 * kBlock), *(const u32x4*)(at + (qat ^ 64) + mt * 16 * kBlock));
   };
-  constexpr int kTail = 2, LAG = 2;
+  constexpr int kTail = 2, LAG = 3;
 
   aim();
   load_next(0);
@@ -684,6 +691,13 @@ __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int 
           asm volatile("" ::: "memory");
         }
         p[i % (LAG + 1)] = Narrow::dot(x[t], q[mt]);
+        // the loads of the block after the next go out between these last products
+        if (i >= (MT - kTail) * 4 && (LINES || b + 1 < a.kb) && d_tile < total) {
+          constexpr int n = kTail * 4;
+          const int k = i - (MT - kTail) * 4;
+#pragma unroll
+          for (int l = k * S::kLoads / n; l < (k + 1) * S::kLoads / n; ++l) load(l, cur);
+        }
         if (i < (MT - kTail) * 4) {
           if (t == 0 && mt + 1 < MT) q[mt + 1] = qr[(mt + 1) & 1];
           if (t == 1 && mt + 2 < MT) qr[mt & 1] = load_q(at, mt + 2);
@@ -696,7 +710,7 @@ __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int 
       }
 #pragma unroll
       for (int i = MT * 4 - LAG; i < MT * 4; ++i) add(i);
-      if (LINES || b + 1 < a.kb) load_next(cur);
+      if ((LINES || b + 1 < a.kb) && d_tile < total) loaded();
       cur ^= 1;
     }
 
