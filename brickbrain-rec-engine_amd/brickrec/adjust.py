@@ -18,7 +18,7 @@ def mask_words(mask: torch.Tensor) -> torch.Tensor:
     """bool [..., n] on a GPU -> int32 words [..., ⌈n/32⌉], bit i of word w = entry 32w + i: the layout of
     ``ItemIndex.eval_mask_bits`` and ``engine.bits_from_bool``, packed on the device."""
     n = mask.shape[-1]
-    pad = torch.nn.functional.pad(mask, (0, -n % 32)).view(*mask.shape[:-1], -1, 32)
+    pad = torch.nn.functional.pad(mask, (0, -n % 32)).view(*mask.shape[:-1], (n + 31) // 32, 32)
     bit = torch.arange(32, device=mask.device)
     return (pad.to(torch.int64) << bit).sum(-1).to(torch.int32)
 
@@ -133,7 +133,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         ids64 = int(bias_ids.dtype is torch.int64)
     if mask is not None:
         if mask.dtype is torch.bool:
-            if mask.shape[-1] != n:
+            if mask.dim() == 0 or mask.shape[-1] != n:
                 raise ValueError(f"a bool mask is [{n}] or [{B}, {n}]: got {tuple(mask.shape)}")
             mask = mask_words(mask)
         mask, w, ld_mask = _list(mask, "mask", _WORDS, B, dev)

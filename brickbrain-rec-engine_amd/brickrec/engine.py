@@ -161,6 +161,7 @@ class ItemIndex:
             L.check(self._lib.bb_destroy(self._h), "bb_destroy")
             self._h = None
         base = getattr(self, "_base", None)
+        self._fp8 = None
         if base is not None:
             with base._mu:
                 base._views -= 1
@@ -534,6 +535,8 @@ class ItemIndex:
         root = getattr(self, "_base", None) or self
         if self.n_items <= 0:
             raise L.BrickrecError("no items uploaded")
+        if chunk < 1:
+            raise ValueError(f"chunk is at least 1: got {chunk}")
         dev = torch.device("cuda", self.device)
         with torch.cuda.device(dev):
             rows = Fp8Rows.empty(self.n_items, self.d, device=dev)
@@ -544,6 +547,11 @@ class ItemIndex:
             torch.cuda.current_stream(dev).synchronize()
         root._fp8 = rows
         return rows
+
+    @property
+    def quantized(self):
+        """The 8-bit copy that ``quantize_items`` made of the items (``fp8.Fp8Rows``), or None."""
+        return getattr(getattr(self, "_base", None) or self, "_fp8", None)
 
     def scores(self, q_rows, *, normalize: bool = True, dtype=None, stream=None, out=None, **adjust):
         """Dense scores [B, n] of query rows against the 8-bit copy of the items (``quantize_items``,
@@ -558,28 +566,35 @@ class ItemIndex:
         import torch
         from .adjust import adjust_scores
         from .fp8 import quantize_rows, scores_fp8
-        root = getattr(self, "_base", None) or self
-        items = getattr(root, "_fp8", None)
+        items = self.quantized
         if items is None:
             raise L.BrickrecError("scores() needs quantize_items() first")
         dev = torch.device("cuda", self.device)
         host = not _is_torch(q_rows)
         if host:
-            q_rows = torch.from_numpy(np.ascontiguousarray(q_rows, dtype=np.float32)).to(dev)
-        if q_rows.dim() != 2 or q_rows.shape[1] != self.d:
+            if dtype not in (None, torch.float32):
+                raise TypeError(f"scores of numpy rows are float32: not {dtype}")
+            q_rows = np.ascontiguousarray(q_rows, dtype=np.float32)
+        elif q_rows.device != dev:
+            raise TypeError(f"query rows are a numpy array or a tensor on {dev}: got one on {q_rows.device}")
+        if q_rows.ndim != 2 or q_rows.shape[1] != self.d:
             raise ValueError(f"query rows are [B, {self.d}]: got {tuple(q_rows.shape)}")
         s = stream if stream is not None else torch.cuda.current_stream(dev)
-        used = [q_rows, items.codes, items.scales] + [t for t in (out, *adjust.values()) if t is not None and _is_torch(t)]
-        for t in used:  # (their memory stays theirs until the stream has passed this call)
-            t.record_stream(s)
+        if s.device != dev:
+            raise ValueError(f"stream of {s.device} for an index on {dev}")
+        for t in (q_rows, items.codes, items.scales, out, *adjust.values()):
+            if _is_torch(t) and t.is_cuda:  # (its memory stays its own until the stream has passed this call)
+                t.record_stream(s)
         with torch.cuda.stream(s):
+            if host:
+                q_rows = torch.from_numpy(q_rows).to(dev)
             q = q_rows.float() if normalize or q_rows.dtype == torch.float64 else q_rows
             if normalize:
                 q = torch.nn.functional.normalize(q, dim=1, eps=1e-30)
             r = scores_fp8(quantize_rows(q), items, dtype=dtype or torch.float32, out=out)
             if adjust:
                 adjust_scores(r, out=r, **adjust)
-        return r.cpu().numpy() if host else r
+            return r.float().cpu().numpy() if host else r
 
     # ------------------------------------------------------------------ options
     def set_option(self, option: str, value: int):

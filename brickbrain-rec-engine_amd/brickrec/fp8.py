@@ -10,6 +10,7 @@ kept between calls.  No gradient flows through these calls, so inputs that ask f
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional
 
 import torch
@@ -73,9 +74,14 @@ def _ld(x: torch.Tensor) -> int:
 class Fp8Rows:
     """``codes`` float8_e4m3fn [n, 128·⌈d/128⌉] (columns from d on zero) and ``scales`` f32
     [⌈d/128⌉, n], or [⌈d/128⌉, ⌈n/128⌉] with ``tile`` (one scale for 128 × 128): element (i, j) is
-    codes[i, j] · scales[j // 128, i or i // 128]."""
+    codes[i, j] · scales[j // 128, i or i // 128].  The calls use the tensors' memory as it is when the
+    rows are made: their contents may change after that, their storage may not be resized or replaced."""
 
-    __slots__ = ("codes", "scales", "d", "tile", "_c")
+    __slots__ = ("_codes", "_scales", "_d", "_tile", "_c")
+    codes = property(operator.attrgetter("_codes"), doc="float8_e4m3fn [n, 128·⌈d/128⌉]")
+    scales = property(operator.attrgetter("_scales"), doc="f32 [⌈d/128⌉, n], or [⌈d/128⌉, ⌈n/128⌉] with tile")
+    d = property(operator.attrgetter("_d"), doc="columns of a row")
+    tile = property(operator.attrgetter("_tile"), doc="whether a scale covers 128 rows")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int, tile: bool = False):
         if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32:
@@ -95,7 +101,8 @@ class Fp8Rows:
             if n > 0 and kb > 0 and (codes.stride(1) != 1 or (sn > 1 and scales.stride(1) != 1)):
                 raise ValueError("codes and scales are contiguous along their rows")
             ld, sld = _ld(codes), _ld(scales)
-        self.codes, self.scales, self.d, self.tile = codes, scales, d, bool(tile)
+        _refuse_grad(codes, scales)
+        self._codes, self._scales, self._d, self._tile = codes, scales, d, bool(tile)
         self._c = L.bb_fp8_rows(codes.data_ptr(), scales.data_ptr(), n, d, ld, sld, 1 if tile else 0)
 
     @classmethod
@@ -105,14 +112,17 @@ class Fp8Rows:
         kb = (d + 127) // 128
         sn = (n + 127) // 128 if tile else n
         new = cls.__new__(cls)
-        new.codes = torch.empty((n, kb * BLOCK), dtype=torch.float8_e4m3fn, device=dev)
-        new.scales = torch.empty((kb, sn), dtype=torch.float32, device=dev)
-        new.d, new.tile = d, bool(tile)
-        new._c = L.bb_fp8_rows(new.codes.data_ptr(), new.scales.data_ptr(), n, d, max(1, kb * BLOCK), max(1, sn), 1 if tile else 0)
+        new._codes = torch.empty((n, kb * BLOCK), dtype=torch.float8_e4m3fn, device=dev)
+        new._scales = torch.empty((kb, sn), dtype=torch.float32, device=dev)
+        new._d, new._tile = d, bool(tile)
+        new._c = L.bb_fp8_rows(new._codes.data_ptr(), new._scales.data_ptr(), n, d, max(1, kb * BLOCK), max(1, sn), 1 if tile else 0)
         return new
 
+    def __reduce__(self):
+        return Fp8Rows, (self._codes, self._scales, self._d, self._tile)
+
     def __len__(self) -> int:
-        return self.codes.shape[0]
+        return self._codes.shape[0]
 
     @property
     def device(self) -> torch.device:
@@ -153,7 +163,7 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
     dev = x.get_device()
     if out is None:
         out = Fp8Rows.empty(n, d, tile, x.device)
-    elif (len(out), out.d, out.tile, out.codes.get_device()) != (n, d, bool(tile), dev):
+    elif (len(out), out._d, out._tile, out._codes.get_device()) != (n, d, bool(tile), dev):
         raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
     rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), C.byref(out._c), _raw_stream(dev))
     if rc:
@@ -167,7 +177,7 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     rounded once to ``dtype`` (f32, bf16 or f16).  The queries' scales are per row; the items' per
     row or per tile.  ``out``: a tensor of that shape (its dtype is then the scores') to write into; its
     rows may be strided, columns behind them stay as they were."""
-    q, x = queries.codes, items.codes
+    q, x = queries._codes, items._codes
     dev = q.get_device()
     if x.get_device() != dev:
         raise ValueError("queries and items are on one device")

@@ -126,7 +126,7 @@ class SemanticIndex:
     def scores(self, queries, **kw):
         """Dense scores [B, n] of query vectors against an 8-bit copy of the embeddings, with penalties,
         biases and masks (``ItemIndex.scores``; the copy is made at the first call)."""
-        if getattr(self.index, "_fp8", None) is None:
+        if self.index.quantized is None:
             self.index.quantize_items()
         q = np.asarray(queries, np.float32) if isinstance(queries, (list, tuple)) else queries
         return self.index.scores(q[None, :] if q.ndim == 1 else q, **kw)

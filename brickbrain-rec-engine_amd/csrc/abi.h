@@ -4,7 +4,6 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
-#include <exception>
 #include <string>
 
 #include "../../include/brickrec.h"

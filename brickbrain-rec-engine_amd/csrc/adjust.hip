@@ -86,13 +86,13 @@ __global__ __launch_bounds__(THREADS) void adjust_kernel(bb_adjust a, int n_chun
     uint32_t* slot = SPLIT ? lds + kChunk : lds;
     if (a.bias_ids) {
       biased.each(biased.n, [&](int e, int64_t id) {
-        const uint64_t at = (uint64_t)(id - c0);
+        const uint64_t at = (uint64_t)id - (uint64_t)c0;  // (ids below the chunk wrap to far above it)
         if (at < (uint64_t)len) atomicMax(&slot[at], SPLIT ? (uint32_t)e + 1u : ((uint32_t)e + 1u) << 16);
       });
       if (!SPLIT && a.seen) __syncthreads();  // (the maxima are over words whose counts are still 0)
     }
     seen.each(n_seen, [&](int, int64_t id) {
-      const uint64_t at = (uint64_t)(id - c0);
+      const uint64_t at = (uint64_t)id - (uint64_t)c0;
       if (at < (uint64_t)len) atomicAdd(&lds[at], 1u);
     });
     __syncthreads();
@@ -160,6 +160,15 @@ int check(const bb_adjust* a) {
   if ((uintptr_t)a->seen % ib || (uintptr_t)a->bias_ids % ib || (uintptr_t)a->seen_len % 4 || (uintptr_t)a->bias % 4 ||
       (uintptr_t)a->mask % 4 || (uintptr_t)a->repetition % 4 || (uintptr_t)a->presence % 4 || (uintptr_t)a->frequency % 4)
     return bad("a list, mask or parameter is not aligned to its type");
+  // what other workgroups may still read
+  auto meets = [&](const void* p, int64_t n, int64_t ld, uint64_t size) {
+    return p && n > 0 && overlap(p, ((uint64_t)(a->B - 1) * ld + n) * size, a->out, o_bytes);
+  };
+  if (meets(a->seen, a->n_seen, a->ld_seen, ib) || meets(a->bias_ids, a->n_bias, a->ld_bias, ib) ||
+      meets(a->bias, a->n_bias, a->ld_bias, 4) || meets(a->mask, (a->n + 31) / 32, a->ld_mask, 4) ||
+      meets(a->seen_len, 1, 1, 4) || meets(a->repetition, 1, 1, 4) || meets(a->presence, 1, 1, 4) ||
+      meets(a->frequency, 1, 1, 4))
+    return bad("out overlaps a list, the mask or a parameter");
   return BB_OK;
 }
 

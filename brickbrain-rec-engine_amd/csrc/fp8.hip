@@ -205,11 +205,6 @@ struct Wide {
 template <typename T>
 using Mode = std::conditional_t<std::is_same_v<T, float>, Wide, Narrow>;
 
-template <typename M>
-__device__ __forceinline__ typename M::Frag load32(const uint8_t* p) {
-  return M::make(*(const u32x4*)p, *(const u32x4*)(p + 16));
-}
-
 // ---- the product of few rows -----------------------------------------------------------------
 // Bound by reading the items once: operands go straight from memory to registers, up to PF blocks
 // of a wave in flight.  A workgroup takes 16 items x 16 queries; its KS waves take every KS-th block of the
@@ -912,6 +907,9 @@ extern "C" int bb_quantize_fp8(int32_t device, const void* x, int32_t dtype, int
     if (ldx < out->d && out->rows > 1) return abi_fail(BB_E_ARG, "bb_quantize_fp8: ldx < d");
     if (meets(out, x, span(out->rows, out->rows > 1 ? ldx : 0, out->d, es)))
       return abi_fail(BB_E_ARG, "bb_quantize_fp8: out overlaps the rows");
+    if (overlap(out->codes, span(out->rows, out->ld, blocks_of(out->d) * kBlock, 1), out->scales,
+                span(blocks_of(out->d), out->scales_ld, out->tile ? blocks_of(out->rows) : out->rows, 4)))
+      return abi_fail(BB_E_ARG, "bb_quantize_fp8: codes and scales overlap");
     CallDevice dev;
     if ((rc = dev.enter(device, "bb_quantize_fp8"))) return rc;
     QuantArgs a{x, ldx, out->rows, out->d, out->codes, out->ld, out->scales, out->scales_ld, (int32_t)blocks_of(out->d)};

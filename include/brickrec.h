@@ -320,7 +320,8 @@ int bb_scores_fp8(int32_t device, const bb_fp8_rows* q, const bb_fp8_rows* items
 typedef struct {
   const void* scores;        /* B x n of `dtype`, ld_scores elements between rows            */
   void* out;                 /* the same shape and type, ld_out between rows; may be scores
-                                itself with the same ld; may not overlap it otherwise        */
+                                itself with the same ld; may not overlap it otherwise, nor
+                                anything else that is read                                   */
   int64_t B, n;
   int64_t ld_scores, ld_out;
   int32_t dtype;             /* BB_F32 / BB_BF16 / BB_F16                                    */

@@ -108,3 +108,19 @@ def test_layouts_match_the_header():
         assert C.sizeof(getattr(L, n)) == lay[n], n
         for f in fields:
             assert getattr(getattr(L, n), f).offset == lay[f"{n}.{f}"], f"{n}.{f}"
+
+
+def test_codes_and_scales_apart():
+    g = rows(scales=(1 << 20) + 2048)
+    err(L.load().bb_quantize_fp8(0, C.c_void_p(1 << 40), L.BB_F32, 200, C.byref(g), None), "codes and scales")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(seen=(1 << 30) + 1024, n_seen=4), dict(seen=(1 << 30) - 4, n_seen=2), dict(mask=1 << 30),
+    dict(bias_ids=1 << 12, bias=(1 << 30) + 8, n_bias=1), dict(bias_ids=(1 << 30) + 8, bias=1 << 12, n_bias=1),
+    dict(seen=1 << 12, n_seen=1, seen_len=(1 << 30) - 8), dict(repetition=1 << 30), dict(presence=1 << 30),
+    dict(frequency=1 << 30), dict(seen=(1 << 30) - 200, n_seen=1, ld_seen=25),
+])
+def test_adjust_out_apart_from_what_is_read(kw):
+    a = adj(**kw)
+    err(L.load().bb_adjust_scores(0, C.byref(a), None), "overlaps a list")

@@ -220,3 +220,36 @@ def test_refusals(br):
     with pytest.raises(ValueError):
         br.adjust_scores(torch.zeros(64, device=DEV))
     assert br.adjust_scores(s[:0]).shape == (0, 64) and br.adjust_scores(s[:, :0]).shape == (3, 0)
+
+
+def test_no_rows_with_every_argument(br):
+    for B, n in ((0, 64), (3, 0), (0, 0)):
+        s = torch.zeros((B, n), device=DEV)
+        y = br.adjust_scores(s, seen=torch.zeros((B, 4), dtype=torch.int32, device=DEV),
+                             seen_len=torch.zeros(B, dtype=torch.int32, device=DEV),
+                             bias_ids=torch.zeros((B, 2), dtype=torch.int32, device=DEV), bias=torch.zeros((B, 2), device=DEV),
+                             mask=torch.ones((B, n), dtype=torch.bool, device=DEV))
+        assert y.shape == (B, n)
+    with pytest.raises(ValueError):
+        br.adjust_scores(s, mask=torch.ones((), dtype=torch.bool, device=DEV))
+
+
+def test_ids_at_the_ends_of_their_type(br):
+    n = 9000
+    a = make(2, n, torch.float32, 8, 4, torch.int64)
+    lo, hi = torch.iinfo(torch.int64).min, torch.iinfo(torch.int64).max
+    a["seen"][:] = torch.tensor([lo, hi, lo + n, -n, n, n - 1, 0, 2 ** 32])
+    a["bias_ids"][:] = torch.tensor([lo, hi, 8192, 2 ** 32 + 1])
+    a["seen_len"][:] = 8
+    check(a, run(br, a))
+
+
+def test_out_over_what_is_read(br):
+    buf = torch.zeros(4 * 64, dtype=torch.int32, device=DEV)
+    out = buf.view(torch.float32).view(4, 64)
+    s = torch.zeros((4, 64), device=DEV)
+    for kw in ({"seen": buf[:8]}, {"seen": buf[-4:]}, {"mask": buf[4:6]}, {"seen": torch.zeros_like(buf[:8]), "seen_len": buf[:4]},
+               {"bias_ids": torch.zeros_like(buf[:8]), "bias": out.view(-1)[8:16]}, {"bias_ids": buf[:8], "bias": s.view(-1)[:8]},
+               {"seen": torch.zeros_like(buf[:8]), "repetition": out.view(-1)[:4]}):
+        with pytest.raises(br.BrickrecError):
+            br.adjust_scores(s, out=out, **kw)

@@ -330,3 +330,101 @@ def test_semantic_scores(br):
     one = sem.scores(x[7].numpy())
     assert one.shape == (1, 500) and int(one[0].argmax()) == 7
     assert np.array_equal(sem.scores([x[7].tolist(), x[8].tolist()])[:1], one)
+
+
+def test_index_scores_refusals_and_streams(br):
+    n, d, B = 70000, 256, 64
+    x, q = make(n, d, seed=1), make(B, d, seed=2)
+    idx = br.ItemIndex()
+    idx.upload_items(x.numpy())
+    assert idx.quantized is None
+    with pytest.raises(ValueError):
+        idx.quantize_items(chunk=0)
+    with pytest.raises(ValueError):
+        idx.quantize_items(chunk=-5)
+    rows = idx.quantize_items()
+    assert idx.quantized is rows
+    with pytest.raises(TypeError):
+        idx.scores(q)                                    # a host tensor
+    with pytest.raises(TypeError):
+        idx.scores(q.numpy(), dtype=torch.bfloat16)      # numpy has no such type
+    with pytest.raises(ValueError):
+        idx.scores(q[:, :100].to(DEV))
+    with pytest.raises(ValueError):
+        idx.scores(q.numpy()[0])
+    want = idx.scores(q.to(DEV)).cpu()
+    assert idx.scores(q[:0].numpy()).shape == (0, n)
+    # numpy rows through another stream that is busy: the copy to the host waits for that one
+    s = torch.cuda.Stream(DEV)
+    a = torch.randn(4096, 4096, device=DEV)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            a = torch.tanh(a @ a)
+    assert torch.equal(torch.from_numpy(idx.scores(q.numpy(), stream=s)), want)
+    # captured and replayed with other queries
+    raw, out = q.to(DEV), torch.zeros((B, n), device=DEV)
+    idx.scores(raw, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        idx.scores(raw, out=out)
+    for i in range(3):
+        raw.copy_(make(B, d, seed=30 + i))
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, idx.scores(raw)), i
+        out.sum().item()
+    del g
+    idx.close()
+    with pytest.raises(br.BrickrecError):
+        idx.scores(raw)
+
+
+def test_rows_keep_their_tensors(br):
+    import copy
+    import io
+    q = quantized(br, 5, 200)
+    for name in ("codes", "scales", "d", "tile"):
+        with pytest.raises(AttributeError):
+            setattr(q, name, None)
+    want = br.scores_fp8(q, q)                           # one set of rows on both sides
+    assert torch.equal(br.scores_fp8(copy.deepcopy(q), q), want)
+    f = io.BytesIO()
+    torch.save(q, f)
+    f.seek(0)
+    with torch.serialization.safe_globals([br.Fp8Rows]):
+        assert torch.equal(br.scores_fp8(q, torch.load(f, weights_only=True)), want)
+    with pytest.raises(ValueError):
+        br.Fp8Rows(q.codes, q.scales.clone().requires_grad_(), 200)
+    with torch.no_grad():
+        br.Fp8Rows(q.codes, q.scales.clone().requires_grad_(), 200)
+
+
+@pytest.mark.parametrize("m, n", [(3, 40), (100, 300), (2100, 8200)])
+def test_two_graphs_at_once(br, m, n):
+    """Two captured calls replayed side by side, each with its own tensors: neither sees the other."""
+    sets = [[quantized(br, m, 384, seed=2 * i), quantized(br, n, 384, seed=2 * i + 1)] for i in range(2)]
+    want = [br.scores_fp8(q, x, dtype=torch.bfloat16) for q, x in sets]
+    outs = [torch.zeros((m, n), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    graphs = []
+    torch.cuda.synchronize()
+    for (q, x), o in zip(sets, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            br.scores_fp8(q, x, out=o)
+            br.adjust_scores(o, out=o, seen=torch.zeros(1, dtype=torch.int32, device=DEV), presence=1.0)
+        graphs.append(g)
+    want = [br.adjust_scores(w, seen=torch.zeros(1, dtype=torch.int32, device=DEV), presence=1.0) for w in want]
+    for _ in range(3):
+        [o.zero_() for o in outs]
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+        outs[0].float().sum().item()
