@@ -539,10 +539,10 @@ __global__ __launch_bounds__(KG* WN* WM * 64, KG* WN* WM > 8 ? KG * WN * WM / 4 
 //  - the loader runs ahead over the tiles' ends, and a tile's scores go out beside the next tile's blocks;
 //  - a product is scaled three products later.  The empty asm keeps the compiler from collecting the sums at the
 //    end of the block, which would hold all 32 products in registers.
-// 4,096 x 8,192 x 4,096: 126 us, 2.18 PFLOP/s (135 us with a workgroup to a tile; 3.2 PFLOP/s is what a large 8-bit
-// product without block scales reaches).  4,096 x 125,000 x 768, whose rows begin anywhere in a line: 664 us against
-// 743 with tiles of 128 and 722 with 128 bytes of a row to a store; from 124,928 items, whose rows begin at
-// lines, 128 bytes take 545 us and 512 take 615.
+// 4,096 x 8,192 x 4,096: 118 us, 2.33 PFLOP/s (135 us with a workgroup to a tile; 3.2 PFLOP/s is what a large 8-bit
+// product without block scales reaches).  4,096 x 125,000 x 768, whose rows begin anywhere in a line: 625 us against
+// 743 with tiles of 128 and 722 with 128 bytes of a row to a store; with 124,992 items, whose rows begin at
+// lines, 128 bytes take 545 us and 512 take 615.  The clock falls to 1.8 to 1.9 GHz under this load (2.4 without).
 template <typename T>
 using RunShape = TileShape<T, 4, 2, 8, 2, 1>;  // 256 x 256
 constexpr int kCus = 256;
@@ -565,25 +565,28 @@ __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int 
   uint32_t xoff[S::kXP], qoff[S::kQP], soff[S::kSP];
   const uint8_t *xb, *qb;
   const float *xsb, *qsb;
+  // (where rows do not begin at lines there are no registers left for what a tile's start and end derive from the
+  // lane: the empty asm has it worked out there instead of kept, and spilled, over the blocks)
   auto aim = [&]() __attribute__((always_inline)) {
-    int tm, tn;
+    int tm, tn, ln = lane;
+    if constexpr (!LINES) asm volatile("" : "+v"(ln));
     tile_of(d_tile, total, tiles_m, tiles_n, tm, tn);
     const int64_t n0 = (int64_t)tn * S::TN, m0 = (int64_t)tm * S::TM;
     const int nx = (int)(a.N - n0 < S::TN ? a.N - n0 : S::TN), nq = (int)(a.M - m0 < S::TM ? a.M - m0 : S::TM);
 #pragma unroll
     for (int p = 0; p < S::kXP; ++p) {
-      const int row = (wave * S::kXP + p) * 8 + (lane >> 3);
-      xoff[p] = (uint32_t)(row < nx ? row : nx - 1) * (uint32_t)a.ldx + (((lane & 7) ^ S::fx(row)) << 4);
+      const int row = (wave * S::kXP + p) * 8 + (ln >> 3);
+      xoff[p] = (uint32_t)(row < nx ? row : nx - 1) * (uint32_t)a.ldx + (((ln & 7) ^ S::fx(row)) << 4);
     }
 #pragma unroll
     for (int p = 0; p < S::kQP; ++p) {
-      const int row = (wave * S::kQP + p) * 8 + (lane >> 3);
-      qoff[p] = (uint32_t)(row < nq ? row : nq - 1) * (uint32_t)a.ldq + (((lane & 7) ^ (row & 7)) << 4);
+      const int row = (wave * S::kQP + p) * 8 + (ln >> 3);
+      qoff[p] = (uint32_t)(row < nq ? row : nq - 1) * (uint32_t)a.ldq + (((ln & 7) ^ (row & 7)) << 4);
     }
 #pragma unroll
     for (int j = 0; j < S::kSP; ++j) {
       const int i = (j * S::kWaves + wave) % ((S::TN + S::TM) / 64);
-      const int row = (i < S::TN / 64 ? i : i - S::TN / 64) * 64 + lane, n = i < S::TN / 64 ? nx : nq;
+      const int row = (i < S::TN / 64 ? i : i - S::TN / 64) * 64 + ln, n = i < S::TN / 64 ? nx : nq;
       const int c = row < n ? row : n - 1;
       soff[j] = (uint32_t)(TILE && i < S::TN / 64 ? c / kBlock : c) * 4;
     }
@@ -756,25 +759,27 @@ __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int 
       constexpr int kRow = S::TN * 2, kHalf = S::TM / 2;
       static_assert(kHalf * kRow <= S::kStage && kRow == 512, "half a tile's scores fit a stage");
       char* turn = smem + (cur ^ 1) * S::kStage;
-      const int c = threadIdx.x & 31;
+      int tid = threadIdx.x;
+      asm volatile("" : "+v"(tid));
+      const int c = tid & 31;
       const int64_t n = (int64_t)tn * S::TN + c * 8;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int i = 0; i < MT / 2; ++i) {
-          char* row = turn + (wm * (kHalf / 2) + i * 16 + r) * kRow;
+          char* row = turn + (wm * (kHalf / 2) + i * 16 + (tid & 15)) * kRow;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             Out v;
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = (T)acc[h * (MT / 2) + i][u * 2 + (j >> 2)][j & 3];
-            *(Out*)(row + (((wn * 8 + u * 4 + g) ^ r) << 4)) = v;
+            *(Out*)(row + (((wn * 8 + u * 4 + (tid >> 4 & 3)) ^ (tid & 15)) << 4)) = v;
           }
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < kHalf / 16; ++i) {
-          const int row = i * 16 + (threadIdx.x >> 5);
+          const int row = i * 16 + (tid >> 5);
           const int64_t m = (int64_t)tm * S::TM + (row / (kHalf / 2)) * (S::TM / 2) + h * (kHalf / 2) + row % (kHalf / 2);
           const Out v = *(const Out*)(turn + row * kRow + ((c ^ (row & 15)) << 4));
           if (m < a.M) {
