@@ -122,10 +122,10 @@ def load() -> C.CDLL:
             "bb_plan_launch": ([P], C.c_int),
             "bb_plan_destroy": ([P], C.c_int),
             "bb_check_dual_scan_args": ([C.c_int64], C.c_int),
-            "bb_quantize_fp8": ([C.c_int32, P, C.c_int32, C.c_int64, C.POINTER(bb_fp8_rows), P], C.c_int),
-            "bb_scores_fp8": ([C.c_int32, C.POINTER(bb_fp8_rows), C.POINTER(bb_fp8_rows), P, C.c_int32, C.c_int64, P],
-                              C.c_int),
-            "bb_adjust_scores": ([C.c_int32, P, P], C.c_int),  # (a bb_adjust by reference, or its bytes)
+            # (a bb_fp8_rows or bb_adjust by reference, or its bytes)
+            "bb_quantize_fp8": ([C.c_int32, P, C.c_int32, C.c_int64, P, P], C.c_int),
+            "bb_scores_fp8": ([C.c_int32, P, P, P, C.c_int32, C.c_int64, P], C.c_int),
+            "bb_adjust_scores": ([C.c_int32, P, P], C.c_int),
             "bb_last_error": ([], C.c_char_p),
             "bb_abi_version": ([], C.c_int),
         }

@@ -9,8 +9,8 @@ kept between calls.  No gradient flows through these calls, so inputs that ask f
 """
 from __future__ import annotations
 
-import ctypes as C
 import operator
+import struct
 from typing import Optional
 
 import torch
@@ -18,6 +18,9 @@ import torch
 from . import _lib as L
 
 BLOCK = 128
+_E4M3, _F32 = torch.float8_e4m3fn, torch.float32
+# bb_fp8_rows packed into bytes (a third of the time of a ctypes structure); its fields in order
+_PACK = struct.Struct("@PPqqqqi4x").pack
 _CODE = {torch.float32: L.BB_F32, torch.bfloat16: L.BB_BF16, torch.float16: L.BB_F16}
 
 
@@ -84,7 +87,7 @@ class Fp8Rows:
     tile = property(operator.attrgetter("_tile"), doc="whether a scale covers 128 rows")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int, tile: bool = False):
-        if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.float32:
+        if codes.dtype is not _E4M3 or scales.dtype is not _F32:
             raise TypeError(f"codes are float8_e4m3fn and scales float32: got {codes.dtype} and {scales.dtype}")
         if not codes.is_cuda or scales.get_device() != codes.get_device():
             raise TypeError("codes and scales are tensors of one GPU")
@@ -101,9 +104,10 @@ class Fp8Rows:
             if n > 0 and kb > 0 and (codes.stride(1) != 1 or (sn > 1 and scales.stride(1) != 1)):
                 raise ValueError("codes and scales are contiguous along their rows")
             ld, sld = _ld(codes), _ld(scales)
-        _refuse_grad(codes, scales)
+        if codes.requires_grad or scales.requires_grad:
+            _refuse_grad(codes, scales)
         self._codes, self._scales, self._d, self._tile = codes, scales, d, bool(tile)
-        self._c = L.bb_fp8_rows(codes.data_ptr(), scales.data_ptr(), n, d, ld, sld, 1 if tile else 0)
+        self._c = _PACK(codes.data_ptr(), scales.data_ptr(), n, d, ld, sld, self._tile)
 
     @classmethod
     def empty(cls, n: int, d: int, tile: bool = False, device=None) -> "Fp8Rows":
@@ -115,7 +119,7 @@ class Fp8Rows:
         new._codes = torch.empty((n, kb * BLOCK), dtype=torch.float8_e4m3fn, device=dev)
         new._scales = torch.empty((kb, sn), dtype=torch.float32, device=dev)
         new._d, new._tile = d, bool(tile)
-        new._c = L.bb_fp8_rows(new._codes.data_ptr(), new._scales.data_ptr(), n, d, max(1, kb * BLOCK), max(1, sn), 1 if tile else 0)
+        new._c = _PACK(new._codes.data_ptr(), new._scales.data_ptr(), n, d, kb * BLOCK or 1, sn or 1, new._tile)
         return new
 
     def __reduce__(self):
@@ -165,7 +169,7 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
         out = Fp8Rows.empty(n, d, tile, x.device)
     elif (len(out), out._d, out._tile, out._codes.get_device()) != (n, d, bool(tile), dev):
         raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
-    rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), C.byref(out._c), _raw_stream(dev))
+    rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), out._c, _raw_stream(dev))
     if rc:
         L.check(rc, "bb_quantize_fp8")
     return out
@@ -192,7 +196,7 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     else:
         _check_out(out, (q.shape[0], x.shape[0]), None, q.device)
         ld = _ld(out)
-    rc = L.load().bb_scores_fp8(dev, C.byref(queries._c), C.byref(items._c), out.data_ptr(), _CODE[out.dtype], ld,
+    rc = L.load().bb_scores_fp8(dev, queries._c, items._c, out.data_ptr(), _CODE[out.dtype], ld,
                                 _raw_stream(dev))
     if rc:
         L.check(rc, "bb_scores_fp8")

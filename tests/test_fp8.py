@@ -124,3 +124,11 @@ def test_codes_and_scales_apart():
 def test_adjust_out_apart_from_what_is_read(kw):
     a = adj(**kw)
     err(L.load().bb_adjust_scores(0, C.byref(a), None), "overlaps a list")
+
+
+def test_rows_packed_as_the_structure():
+    from brickrec import fp8
+    b = fp8._PACK(1 << 20, 1 << 30, 10, 200, 256, 11, True)
+    r = L.bb_fp8_rows.from_buffer_copy(b)
+    assert len(b) == C.sizeof(r)
+    assert [getattr(r, f[0]) for f in r._fields_] == [1 << 20, 1 << 30, 10, 200, 256, 11, 1]
