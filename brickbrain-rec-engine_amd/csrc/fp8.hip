@@ -860,12 +860,27 @@ int launch_product(const ProductArgs& a, void* stream) {
   }
   // 64 x 8,192 x 4,096 10.9 us against 13.0 unsplit, 128 x 2,048 x 8,192 17.4 against 23.2
   if (split) return launch_tile<T, 1, 4, 1, 2, 4>(a, stream);
-  // 40 x 100,000 x 384 f32 14.6 us against 18.6 with tiles of 128; 128 x 25,216 x 384 f32 (197 tiles) 8.8 against 8.2
-  if (a.M <= 64 || tiles(a, 128) < 192) return launch_tile<T, 1, 4, 1, 2, 1>(a, stream);
+  if (a.M <= 64 || tiles(a, 128) < 192) {
+    // three stages where no CU has more than two workgroups, so that there is LDS for them, and rows are long:
+    // 128 x 16,384 x 4,096 16.8 us against 19.7, 64 x 32,768 x 8,192 57.5 against 64.7; 64 x 65,536 x 2,048 (four
+    // a CU) 31.7 against 30.0, 64 x 30,000 x 1,536 10.7 against 10.2; f32 scores are bound by the matrix cores
+    if constexpr (sizeof(T) == 2) {
+      if (a.kb >= 16 && tiles(a, 64) <= 2 * kCus) return launch_tile<T, 1, 4, 1, 3, 1>(a, stream);
+    }
+    // 40 x 100,000 x 384 f32 14.6 us against 18.6 with tiles of 128; 256 x 8,192 x 512 (128 tiles) 4.9 against 6.4
+    return launch_tile<T, 1, 4, 1, 2, 1>(a, stream);
+  }
+  // About one tile of 128 a CU: halves of them, two workgroups to a CU, overlap.  333 x 10,007 x 1,000 f16 (237 tiles) 9.6 us
+  // against 11.6, 512 x 8,192 x 4,096 (256) 23.6 against 27.0, 300 x 12,000 x 384 (282) 6.6 against 7.5, 128 x 25,216 x 384 f32
+  // (197) 7.7 against 8.2; 768 x 8,192 x 4,096 (384) 36.0 against 35.0, 512 x 16,384 x 768 (512) 13.7 against 12.2
+  if (4 * tiles(a, 128) <= 5 * kCus) return launch_tile<T, 1, 4, 2, 2, 1>(a, stream);
   if constexpr (sizeof(T) == 2) {
     // rounds over the chip: one 256 x 256 tile a CU takes 1.8 times what two 128 x 128 tiles a CU do (4,096 x 8,192 x 4,096:
-    // 2 rounds 126 us against 4 rounds 145; 1,024 x 8,192 x 8,192: half a round 98 us against one 74)
-    if (9 * up(tiles(a, 256), kCus) <= 5 * up(tiles(a, 128), 2 * kCus)) return launch_run<T>(a, stream);
+    // 2 rounds 118 us against 4 rounds 135; 1,024 x 8,192 x 8,192: half a round 98 us against one 74).  A single
+    // round has no tile after it to overlap with, and pays for long rows alone (2,048 x 8,192 x 4,096 63.5 us against
+    // 76.0, x 512 18.2 against 16.7; 333 x 25,216 x 384 14.9 against 10.8)
+    const int64_t rounds = up(tiles(a, 256), kCus);
+    if (9 * rounds <= 5 * up(tiles(a, 128), 2 * kCus) && (rounds > 1 || a.kb >= 12)) return launch_run<T>(a, stream);
   }
   return launch_tile<T, 2, 2, 4, 2, 1>(a, stream);
 }

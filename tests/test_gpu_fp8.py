@@ -428,3 +428,16 @@ def test_two_graphs_at_once(br, m, n):
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
         outs[0].float().sum().item()
+
+
+# sizes on both sides of the rules that choose how the product is cut up
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k, ld", [(4090, 8100, 100, 8100), (4090, 8100, 100, 8192), (2040, 8190, 1600, 8190), (2040, 8190, 1500, 8192),
+                                         (333, 10007, 1000, 10007), (256, 20001, 260, 20032), (130, 14900, 2100, 14900),
+                                         (64, 20001, 2048, 20001), (100, 16300, 2200, 16300), (1000, 7100, 770, 7100)])
+def test_scores_cut_up(br, m, n, k, ld, dtype, tile):
+    q, x = quantized(br, m, k, seed=3), quantized(br, n, k, tile, seed=4)
+    buf = torch.full((m, ld), float("nan"), dtype=dtype, device=DEV)
+    check_scores(q, x, br.scores_fp8(q, x, out=buf[:, :n]), DEV)
+    assert bool(torch.isnan(buf[:, n:]).all())
