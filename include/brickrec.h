@@ -282,7 +282,8 @@ int bb_check_dual_scan_args(int64_t ldx);
  * These calls need no index: every pointer is a device pointer on `device` (-1 = the current
  * device), and the work goes out on `stream` (a hipStream_t; NULL = the null stream) without a
  * synchronisation, an allocation, a fill or a copy, so a call can be captured into a graph.  They
- * keep no state between calls and may run from several threads. */
+ * keep no state between calls and may run from several threads.  A call is one launch; one that
+ * would need 2^32 threads or more (2^28 blocks to quantise, 2^35 scores to adjust) is refused. */
 
 /* Rows of 8-bit floating point (e4m3: 448 the largest, no infinities) with an f32 scale for
  * each block: element (i, j) is codes[i*ld + j] * scales[(j/128)*scales_ld + i], or with

@@ -253,3 +253,24 @@ def test_out_over_what_is_read(br):
                {"seen": torch.zeros_like(buf[:8]), "repetition": out.view(-1)[:4]}):
         with pytest.raises(br.BrickrecError):
             br.adjust_scores(s, out=out, **kw)
+
+
+@pytest.mark.parametrize("B, n", [(1, 33), (6, 9000), (64, 131072)])
+def test_replayed_with_a_bool_mask(br, B, n):
+    """The words of a bool mask are made by a few more launches: captured with the call, replayed with other masks."""
+    scores = torch.randn((B, n), device=DEV)
+    mask = torch.ones((B, n), dtype=torch.bool, device=DEV)
+    out = torch.zeros_like(scores)
+    br.adjust_scores(scores, out=out, mask=mask)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        br.adjust_scores(scores, out=out, mask=mask)
+    for s in range(4):
+        m = torch.rand((B, n), generator=torch.Generator().manual_seed(s)) < 0.5
+        mask.copy_(m)
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, scores.masked_fill(~mask, -INF)), s
+        out.clamp(min=0).sum().item()
