@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib as L
-from .fp8 import _CODE, _On, _check_out, _ld, _raw_stream, _refuse_grad, _rows_of
+from .fp8 import _CODE, _On, _check_out, _empty, _ld, _raw_stream, _refuse_grad, _rows_of
 
 Number = Union[float, torch.Tensor]
 
@@ -27,6 +27,7 @@ def mask_words(mask: torch.Tensor) -> torch.Tensor:
 _PACK = struct.Struct("@PPqqqqiiPqqPPPPfffPPqqPq").pack
 _IDS = {torch.int32: 0, torch.int64: 1}
 _F32 = {torch.float32: 0}
+_FLOAT, _BOOL = torch.float32, torch.bool
 _WORDS = {torch.int32: 0, torch.uint32: 0}
 
 
@@ -35,9 +36,10 @@ def _list(t, name, dtypes, B, dev):
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.get_device() != dev:
         raise TypeError(f"{name} is a tensor of {' or '.join(str(d) for d in dtypes)} on cuda:{dev}")
     shape = t.shape
+    flat = t.is_contiguous()
     if len(shape) == 2 and shape[0] == B:
         m = shape[1]
-        if t.is_contiguous():
+        if flat:
             return t, m, m or 1
         if t.stride(0) == 0 and t.stride(1) == 1:  # one list expanded over the rows
             return t, m, 0
@@ -45,18 +47,19 @@ def _list(t, name, dtypes, B, dev):
         return t, m, _ld(t)
     if len(shape) != 1:
         raise ValueError(f"{name} is [{B}, m] or [m]: got {tuple(shape)}")
-    return t.contiguous(), shape[0], 0
+    return t if flat else t.contiguous(), shape[0], 0
 
 
 def _per_row(v: Number, name, B, dev):
     """A value for all rows, or a tensor of one for each -> (pointer or 0, value, tensor)."""
     if not isinstance(v, torch.Tensor):
         return 0, float(v), None
-    if v.dtype is not torch.float32 or v.get_device() != dev or tuple(v.shape) != (B,):
+    if v.dtype is not _FLOAT or v.get_device() != dev or v.dim() != 1 or v.numel() != B:
         raise TypeError(f"{name} is a number or a float32 tensor [{B}] on cuda:{dev}")
     if v.requires_grad:
         _refuse_grad(v)
-    v = v.contiguous()
+    if not v.is_contiguous():
+        v = v.contiguous()
     return v.data_ptr(), 0.0, v
 
 
@@ -87,15 +90,16 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
                                  frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, out=out)
     if scores.requires_grad:
         _refuse_grad(scores)
-    B, n = scores.shape
-    dev = scores.get_device()
-    scores = _rows_of(scores)
+    shape, dtype, dev = scores.shape, scores.dtype, scores.get_device()
+    B, n = shape
+    ld_scores = ld = n or 1
+    if not scores.is_contiguous():
+        scores = _rows_of(scores)
+        ld_scores = _ld(scores)
     if out is None:
-        out = torch.empty((B, n), dtype=scores.dtype, device=scores.device)
-        ld = max(1, n)
+        out = _empty(B, n, dtype, scores.device)
     else:
-        _check_out(out, (B, n), scores.dtype, scores.device)
-        ld = _ld(out)
+        ld = _check_out(out, shape, dtype, dev)
     # every tensor that the launch reads has a name here until it is out
     seen_p = seen_len_p = rep_p = pre_p = fre_p = bias_ids_p = bias_p = mask_p = 0
     n_seen = ld_seen = n_bias = ld_bias = ld_mask = ids64 = 0
@@ -108,9 +112,10 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         seen, n_seen, ld_seen = _list(seen, "seen", _IDS, B, dev)
         seen_p, ids64 = seen.data_ptr(), int(seen.dtype is torch.int64)
         if seen_len is not None:
-            if seen_len.dtype is not torch.int32 or seen_len.get_device() != dev or seen_len.dim() != 1 or seen_len.shape[0] != B:
+            if seen_len.dtype is not torch.int32 or seen_len.get_device() != dev or seen_len.dim() != 1 or seen_len.numel() != B:
                 raise TypeError(f"seen_len is an int32 tensor [{B}] on cuda:{dev}")
-            seen_len = seen_len.contiguous()
+            if not seen_len.is_contiguous():
+                seen_len = seen_len.contiguous()
             seen_len_p = seen_len.data_ptr()
         rep_p, rep, repetition = _per_row(repetition, "repetition", B, dev)
         pre_p, pre, presence = _per_row(presence, "presence", B, dev)
@@ -132,7 +137,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         bias_ids_p, bias_p = bias_ids.data_ptr(), bias.data_ptr()
         ids64 = int(bias_ids.dtype is torch.int64)
     if mask is not None:
-        if mask.dtype is torch.bool:
+        if mask.dtype is _BOOL:
             if mask.dim() == 0 or mask.shape[-1] != n:
                 raise ValueError(f"a bool mask is [{n}] or [{B}, {n}]: got {tuple(mask.shape)}")
             mask = mask_words(mask)
@@ -141,7 +146,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
             raise ValueError(f"the mask of {n} scores has {(n + 31) // 32} words: got {w}")
         mask_p = mask.data_ptr()
     rc = L.load().bb_adjust_scores(
-        dev, _PACK(scores.data_ptr(), out.data_ptr(), B, n, _ld(scores), ld, _CODE[scores.dtype], ids64, seen_p, n_seen, ld_seen,
+        dev, _PACK(scores.data_ptr(), out.data_ptr(), B, n, ld_scores, ld, _CODE[dtype], ids64, seen_p, n_seen, ld_seen,
                    seen_len_p, rep_p, pre_p, fre_p, rep, pre, fre, bias_ids_p, bias_p, n_bias, ld_bias, mask_p, ld_mask),
         _raw_stream(dev))
     if rc:
