@@ -441,3 +441,16 @@ def test_scores_cut_up(br, m, n, k, ld, dtype, tile):
     buf = torch.full((m, ld), float("nan"), dtype=dtype, device=DEV)
     check_scores(q, x, br.scores_fp8(q, x, out=buf[:, :n]), DEV)
     assert bool(torch.isnan(buf[:, n:]).all())
+
+
+@pytest.mark.parametrize("far_side", ["items", "queries"])
+def test_offsets_within_a_tile_past_31_bits(br, far_side):
+    # 256 rows just under 2^24 bytes apart, in one tile of 256: offsets up to nearly 2^32
+    ld = (1 << 24) - 16
+    store = torch.empty(255 * ld + 128, dtype=torch.uint8, device=DEV)
+    far = torch.as_strided(store, (256, 128), (ld, 1)).view(torch.float8_e4m3fn)
+    near, many = quantized(br, 256, 128, seed=4), quantized(br, 131072, 128, seed=5)
+    far.copy_(near.codes)
+    rows = br.Fp8Rows(far, near.scales, 128)
+    a, b = ((many, rows), (many, near)) if far_side == "items" else ((rows, many), (near, many))
+    assert torch.equal(br.scores_fp8(*a, dtype=torch.bfloat16), br.scores_fp8(*b, dtype=torch.bfloat16))
