@@ -167,13 +167,13 @@ struct ProductArgs {
 // 4 (l >> 4) + j of the first operand against row l & 15 of the second.
 //
 // Two ways, chosen by the type of the scores:
-//  - 16-bit scores: v_mfma_f32_16x16x128_f8f6f4 on the codes as they are.  It cuts each product of a
-//    group of 8 (8 consecutive bytes of a lane) at 2^-13 of the group's largest before it sums
-//    them in f32 (measured: the instruction's rounding is not documented; every 8-bit form does the
-//    same), an error of 1.4e-5 of the result on normal inputs and at most 2^-10 of the sum of magnitudes.  bf16
-//    rounds the result by 2^-8, f16 by 2^-11.
-//  - f32 scores: the codes widened to f16, which holds every e4m3 value, and v_mfma_f32_16x16x32_f16,
-//    which keeps 24 bits under the largest product (2.9e-9 on the same inputs), at half the rate.
+//  - bf16 scores: v_mfma_f32_16x16x128_f8f6f4 on the codes as they are.  It cuts each product of a group of 8
+//    (8 consecutive bytes of a lane) at 2^-13 of the group's largest before it sums them in f32 (measured:
+//    the instruction's rounding is not documented; every 8-bit form does the same), an error of 1.4e-5 of the result
+//    on normal inputs and at most 8 * 2^-13 = 2^-10 of the sum of magnitudes: a quarter of bf16's own half step 2^-8.
+//  - f32 and f16 scores, whose half steps 2^-24 and 2^-11 are finer than that bound: the codes widened to f16, which
+//    holds every e4m3 value, and v_mfma_f32_16x16x32_f16, which keeps 24 bits under the largest product (2.9e-9 on
+//    the same inputs), at half the rate.
 struct Narrow {
   typedef i32x8 Frag;
   static __device__ __forceinline__ Frag make(u32x4 lo, u32x4 hi) {
@@ -205,7 +205,7 @@ struct Wide {
   }
 };
 template <typename T>
-using Mode = std::conditional_t<std::is_same_v<T, float>, Wide, Narrow>;
+using Mode = std::conditional_t<std::is_same_v<T, __bf16>, Narrow, Wide>;
 
 // ---- the product of few rows -----------------------------------------------------------------
 // Bound by reading the items once: operands go straight from memory to registers, up to PF blocks
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(KG* WN* WM * 64, KG* WN* WM > 8 ? KG * WN * WM / 4 
   }
 }
 
-// ---- 16-bit scores of many rows: one workgroup a CU, tile after tile --------------------------------
+// ---- bf16 scores of many rows: one workgroup a CU, tile after tile --------------------------------
 // Tiles of 256 x 256, 8 waves of 64 items x 128 queries, two stages.  What the LDS has to deliver bounds it
 // (192 KB a block to the 8 waves, beside 64 KB that come in), then the matrix cores, then the scaling (4 or 8
 // FMA slots beside each product of 16 x 16 x 128).  Hence:
@@ -555,7 +555,7 @@ template <typename T, bool TILE, bool LINES>
 __global__ __launch_bounds__(512, 2) void product_run_kernel(ProductArgs a, int tiles_m, int tiles_n) {
   using S = RunShape<T>;
   constexpr int V = S::V, WN = 4, MT = 8;
-  static_assert(V == 2 && S::kThreads == 512, "16-bit scores");
+  static_assert(std::is_same_v<Mode<T>, Narrow> && V == 2 && S::kThreads == 512, "bf16 scores");
   constexpr int kOwn = LINES ? 16 * 64 * 2 : 0;  // a wave's 16 x 64 scores
   static_assert(2 * S::kStage + S::kWaves * kOwn <= 160 * 1024, "the stages and the waves' turning places fit the LDS");
   __shared__ __attribute__((aligned(1024))) char smem[2 * S::kStage + S::kWaves * kOwn];
@@ -867,18 +867,20 @@ int launch_product(const ProductArgs& a, void* stream) {
   if (a.M <= 64 || tiles(a, 128) < 192) {
     // three stages where no CU has more than two workgroups, so that there is LDS for them, and rows are long:
     // 128 x 16,384 x 4,096 16.8 us against 19.7, 64 x 32,768 x 8,192 57.5 against 64.7; 64 x 65,536 x 2,048 (four
-    // a CU) 31.7 against 30.0, 64 x 30,000 x 1,536 10.7 against 10.2; f32 scores are bound by the matrix cores
-    if constexpr (sizeof(T) == 2) {
+    // a CU) 31.7 against 30.0, 64 x 30,000 x 1,536 10.7 against 10.2; f32 and f16 scores are bound by the matrix cores (12.9
+    // against 13.6)
+    if constexpr (std::is_same_v<T, __bf16>) {
       if (a.kb >= 16 && tiles(a, 64) <= 2 * kCus) return launch_tile<T, 1, 4, 1, 3, 1>(a, stream);
     }
     // 40 x 100,000 x 384 f32 14.6 us against 18.6 with tiles of 128; 256 x 8,192 x 512 (128 tiles) 4.9 against 6.4
     return launch_tile<T, 1, 4, 1, 2, 1>(a, stream);
   }
-  // About one tile of 128 a CU: halves of them, two workgroups to a CU, overlap.  333 x 10,007 x 1,000 f16 (237 tiles) 9.6 us
-  // against 11.6, 512 x 8,192 x 4,096 (256) 23.6 against 27.0, 300 x 12,000 x 384 (282) 6.6 against 7.5, 128 x 25,216 x 384 f32
-  // (197) 7.7 against 8.2; 768 x 8,192 x 4,096 (384) 36.0 against 35.0, 512 x 16,384 x 768 (512) 13.7 against 12.2
+  // About one tile of 128 a CU: halves of them, two workgroups to a CU, overlap.  333 x 10,007 x 1,000 (237 tiles) bf16 9.7 us
+  // against 11.2, f16 13.2 against 14.0, 512 x 8,192 x 4,096 (256) bf16 24.2 against 28.0, f16 41.1 against 39.8,
+  // 300 x 12,000 x 384 (282) 6.5 against 7.4, 128 x 25,216 x 384 f32 (197) 7.8 against 8.0; 768 x 8,192 x 4,096 (384) bf16
+  // 36.0 against 35.0, f16 61.4 against 58.9, 512 x 16,384 x 768 (512) bf16 13.7 against 12.2, f16 18.2 against 14.9
   if (4 * tiles(a, 128) <= 5 * kCus) return launch_tile<T, 1, 4, 2, 2, 1>(a, stream);
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (std::is_same_v<T, __bf16>) {
     // rounds over the chip: one 256 x 256 tile a CU takes 1.8 times what two 128 x 128 tiles a CU do (4,096 x 8,192 x 4,096:
     // 2 rounds 118 us against 4 rounds 135; 1,024 x 8,192 x 8,192: half a round 98 us against one 74).  A single
     // round has no tile after it to overlap with, and pays for long rows alone (2,048 x 8,192 x 4,096 63.5 us against

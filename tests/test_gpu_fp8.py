@@ -454,3 +454,45 @@ def test_offsets_within_a_tile_past_31_bits(br, far_side):
     rows = br.Fp8Rows(far, near.scales, 128)
     a, b = ((many, rows), (many, near)) if far_side == "items" else ((rows, many), (near, many))
     assert torch.equal(br.scores_fp8(*a, dtype=torch.bfloat16), br.scores_fp8(*b, dtype=torch.bfloat16))
+
+
+# one size for each way the product is cut up, in bf16 and in the wider types
+WAYS = [(1, 300, 384), (16, 40, 2304), (20, 6000, 128), (64, 4100, 1024), (60, 20100, 2048), (250, 8100, 384), (1000, 7100, 384),
+        (2040, 8190, 300)]
+
+
+def small_codes(n, k, seed):
+    """Codes of 0, +-1 and +-2."""
+    return torch.randint(-2, 3, (n, -(-k // 128) * 128), generator=torch.Generator().manual_seed(seed)).float()
+
+
+def rows_of_codes(br, codes, exponents=0.0):
+    n, k = codes.shape
+    scales = torch.full((k // 128, n), 2.0) ** exponents
+    return br.Fp8Rows(codes.to(torch.float8_e4m3fn).to(DEV), scales.float().to(DEV), k)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_small_products_beside_large_ones_that_cancel(br, m, n, k, dtype):
+    """In every 8 columns two products of 448 x 448 cancel and six of at most 4 are left.  Every product is a whole number
+    and every partial sum of a block is below 2^24, so f32 sums are exact; the result is at most 4 * 6 * 16 a block, over at
+    most 18 blocks.  f32 holds it; f16 rounds it once."""
+    q, x = small_codes(m, k, 1), small_codes(n, k, 2)
+    q[:, ::8], q[:, 1::8], x[:, ::8], x[:, 1::8] = 448.0, 448.0, 448.0, -448.0
+    want = (q.double().to(DEV) @ x.double().to(DEV).t().contiguous()).to(dtype)
+    assert torch.equal(br.scores_fp8(rows_of_codes(br, q), rows_of_codes(br, x), dtype=dtype), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, n, k", WAYS)
+def test_exact_sums_are_rounded_once(br, m, n, k, dtype):
+    """Products of 0, 1, 2 and 4 lie within 2^-2 of each other, so that no type's way cuts any of them: blocks are whole
+    numbers of at most 512, scaled by 2^-3 to 2^3, so that every sum has at most 20 bits and the one rounding is left."""
+    q, x = small_codes(m, k, 3), small_codes(n, k, 4)
+    g = torch.Generator().manual_seed(5)
+    eq = torch.randint(-1, 2, (q.shape[1] // 128, m), generator=g)
+    ex = torch.randint(-2, 3, (x.shape[1] // 128, n), generator=g)
+    a, b = rows_of_codes(br, q, eq), rows_of_codes(br, x, ex)
+    want = R.values(a.codes, a.scales).to(DEV) @ R.values(b.codes, b.scales).to(DEV).t().contiguous()
+    assert torch.equal(br.scores_fp8(a, b, dtype=dtype), want.to(dtype))
