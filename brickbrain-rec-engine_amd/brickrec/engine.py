@@ -57,6 +57,19 @@ def _null(stream) -> int:
     return L.BB_Q_NULL_STREAM if int(stream.cuda_stream) == 0 else 0
 
 
+def _unit_rows(q):
+    """f32 or f64 torch rows, L2-normalised in their own type (zero rows stay zero).  Each row is first divided by
+    the power of two in its largest magnitude, so that no square overflows or vanishes; that division is
+    exact and changes no bit of rows whose squares would not have done so."""
+    import torch
+    word, exponent, least = {torch.float32: (torch.int32, 0x7F800000, 2.0 ** -126),
+                             torch.float64: (torch.int64, 0x7FF0000000000000, 2.0 ** -1022)}[q.dtype]
+    top = torch.linalg.vector_norm(q, float("inf"), dim=1, keepdim=True)
+    power = (top.view(word) & exponent).view(q.dtype).clamp_min_(least)
+    # (the norm of a row that is not zero is now at least 1, or 2^-23 (2^-52) for the smallest numbers)
+    return torch.nn.functional.normalize(q / power, dim=1, eps=1e-30)
+
+
 def _torch_dtype_code(t) -> int:
     import torch
     return {torch.float32: L.BB_F32, torch.float64: L.BB_F64, torch.bfloat16: L.BB_BF16}[t.dtype]
@@ -556,7 +569,8 @@ class ItemIndex:
     def scores(self, q_rows, *, normalize: bool = True, dtype=None, stream=None, out=None, **adjust):
         """Dense scores [B, n] of query rows against the 8-bit copy of the items (``quantize_items``,
         called first): column j is item id_offset + j.  The queries are L2-normalised unless
-        ``normalize`` is False (a zero row scores 0), then quantised as the items are; the scores
+        ``normalize`` is False (in their own type, f64 rows in f64, others in f32; a zero row scores 0), then quantised
+        as the items are; the scores
         are those of the 8-bit rows, not the exact ones that ``search`` ranks by.  ``adjust``: the
         penalties, biases and mask of ``adjust.adjust_scores``, applied in place.  Every stored row gets
         a score; pass a mask to leave rows out.
@@ -574,7 +588,9 @@ class ItemIndex:
         if host:
             if dtype not in (None, torch.float32):
                 raise TypeError(f"scores of numpy rows are float32: not {dtype}")
-            q_rows = np.ascontiguousarray(q_rows, dtype=np.float32)
+            q_rows = np.ascontiguousarray(q_rows)
+            if q_rows.dtype not in (np.float32, np.float64):
+                q_rows = q_rows.astype(np.float64 if normalize else np.float32)
         elif q_rows.device != dev:
             raise TypeError(f"query rows are a numpy array or a tensor on {dev}: got one on {q_rows.device}")
         if q_rows.ndim != 2 or q_rows.shape[1] != self.d:
@@ -588,9 +604,11 @@ class ItemIndex:
         with torch.cuda.stream(s):
             if host:
                 q_rows = torch.from_numpy(q_rows).to(dev)
-            q = q_rows.float() if normalize or q_rows.dtype == torch.float64 else q_rows
+            q = q_rows
             if normalize:
-                q = torch.nn.functional.normalize(q, dim=1, eps=1e-30)
+                q = _unit_rows(q if q.dtype in (torch.float32, torch.float64) else q.float())
+            if q.dtype == torch.float64:
+                q = q.float()
             r = scores_fp8(quantize_rows(q), items, dtype=dtype or torch.float32, out=out)
             if adjust:
                 adjust_scores(r, out=r, **adjust)

@@ -12,6 +12,7 @@ import _fp8_ref as R
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda", 0)
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
+INF = float("inf")
 
 
 @pytest.fixture(scope="module")
@@ -496,3 +497,34 @@ def test_exact_sums_are_rounded_once(br, m, n, k, dtype):
     a, b = rows_of_codes(br, q, eq), rows_of_codes(br, x, ex)
     want = R.values(a.codes, a.scales).to(DEV) @ R.values(b.codes, b.scales).to(DEV).t().contiguous()
     assert torch.equal(br.scores_fp8(a, b, dtype=dtype), want.to(dtype))
+
+
+def test_index_scores_of_any_magnitude(br):
+    """Queries are normalised whatever their magnitude: a power of two in front changes nothing, in f32 up to where
+    squares leave its range on either side, in f64 beyond f32's range altogether."""
+    n, d, B = 700, 384, 5
+    idx = br.ItemIndex()
+    idx.upload_items(make(n, d, seed=1).numpy())
+    idx.quantize_items()
+    q = make(B, d, seed=2)
+    want = idx.scores(q.to(DEV))
+    for e in (66, 120, -66, -83, -110):
+        assert torch.equal(idx.scores((q * 2.0 ** e).to(DEV)), want), e
+    wide = idx.scores(q.double().to(DEV))
+    cos = torch.nn.functional.normalize(q.double(), dim=1) @ torch.from_numpy(idx.get_rows(np.arange(n))).double().t()
+    for got in (want, wide):  # (the bound of test_index_scores)
+        assert float((got.cpu().double() - cos).abs().max()) < 2 * 2.0 ** -4 + 2.0 ** -7
+    for e in (600, -600, 1010, -1000):
+        assert torch.equal(idx.scores((q.double() * 2.0 ** e).to(DEV)), wide), e
+        assert np.array_equal(idx.scores((q.double() * 2.0 ** e).numpy()), wide.cpu().numpy()), e
+    # the smallest power of two and the largest, zeros, infinities and NaN
+    q = torch.zeros((6, d))
+    q[0], q[1, 3], q[2] = 2.0 ** -149, 2.0 ** -149, 2.0 ** 127
+    q[4, 7], q[5, 9] = INF, float("nan")
+    got = idx.scores(q.to(DEV))
+    one = torch.zeros((2, d))
+    one[0], one[1, 3] = 1.0, 1.0
+    assert torch.equal(got[[0, 2]], idx.scores(one[[0, 0]].to(DEV)))
+    assert torch.equal(got[1], idx.scores(one[1:].to(DEV))[0])
+    assert bool((got[3] == 0).all()) and bool(torch.isnan(got[4:]).all())
+    idx.close()
