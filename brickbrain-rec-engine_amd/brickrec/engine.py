@@ -542,23 +542,25 @@ class ItemIndex:
     def quantize_items(self, chunk: int = 65536):
         """An 8-bit copy of the stored (normalised) rows, kept with this index and its views until the
         next upload: 1 byte an element and 4 for each 128 of a row.  Returns it (``fp8.Fp8Rows``).
-        Synchronous, as an upload is."""
+        Synchronous, as an upload is; an upload from another thread waits for it."""
         import torch
         from .fp8 import Fp8Rows, quantize_rows
         root = getattr(self, "_base", None) or self
-        if self.n_items <= 0:
-            raise L.BrickrecError("no items uploaded")
         if chunk < 1:
             raise ValueError(f"chunk is at least 1: got {chunk}")
         dev = torch.device("cuda", self.device)
-        with torch.cuda.device(dev):
-            rows = Fp8Rows.empty(self.n_items, self.d, device=dev)
-            for a in range(0, self.n_items, chunk):
-                b = min(self.n_items, a + chunk)
-                ids = torch.arange(self.id_offset + a, self.id_offset + b, device=dev)
-                quantize_rows(self.get_rows(ids), out=rows.part(a, b))
+        # (the rows stay the same from the first chunk until their copy is in its place; through a view too the root's
+        # lock is the only one taken)
+        with root._mu, torch.cuda.device(dev):
+            n, off = root.n_items, root.id_offset
+            if n <= 0:
+                raise L.BrickrecError("no items uploaded")
+            rows = Fp8Rows.empty(n, root.d, device=dev)
+            for a in range(0, n, chunk):
+                b = min(n, a + chunk)
+                quantize_rows(root.get_rows(torch.arange(off + a, off + b, device=dev)), out=rows.part(a, b))
             torch.cuda.current_stream(dev).synchronize()
-        root._fp8 = rows
+            root._fp8 = rows
         return rows
 
     @property

@@ -1,7 +1,13 @@
 """The host side of the dense scores, without a GPU."""
+import contextlib
+import threading
+import types
+
+import numpy as np
 import pytest
 import torch
 
+from brickrec import _lib as L
 from brickrec import engine
 
 
@@ -22,3 +28,65 @@ def test_rows_of_any_magnitude_are_normalised(dtype):
     # 4 equal numbers: squares below 4, their sum, its root and the quotient each off by at most half a step
     assert bool(((got[1] - 0.5).abs() <= 4 * f.eps).all())
     assert bool(torch.isnan(got[3:]).any(1).all())
+
+
+class _Lib:
+    """What the index's calls reach here, with the library's status codes."""
+
+    def __init__(self, rc=0):
+        self.rc = rc
+
+    def bb_upload_items(self, *a):
+        return self.rc
+
+    def bb_last_error(self):
+        return b"stub"
+
+
+def _index(monkeypatch, n=10, d=8):
+    """An index whose rows are host tensors, and whose 8-bit copies are made by nothing."""
+    from brickrec import fp8
+
+    class Rows:
+        def __init__(self, n=n, d=d, **kw):
+            self.got = []
+
+        def part(self, a, b):
+            return self.got
+
+    idx = engine.ItemIndex.__new__(engine.ItemIndex)
+    idx._lib, idx._h, idx._mu = _Lib(), None, threading.RLock()
+    idx.dtype, idx.device, idx.id_offset, idx.n_items, idx.d = "f32", 0, 0, n, d
+    real = torch.arange
+    monkeypatch.setattr(torch, "arange", lambda *a, device=None: real(*a))
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: types.SimpleNamespace(synchronize=lambda: None))
+    monkeypatch.setattr(fp8.Fp8Rows, "empty", staticmethod(Rows))
+    monkeypatch.setattr(fp8, "quantize_rows", lambda x, out: out.append(x))
+    idx.get_rows = lambda ids: ids
+    return idx
+
+
+@pytest.mark.parametrize("through_view", [False, True])
+@pytest.mark.parametrize("at", [0, 8])
+def test_an_upload_waits_for_the_copy_and_drops_it(monkeypatch, at, through_view):
+    idx = _index(monkeypatch)
+    other = None
+
+    def get_rows(ids):
+        nonlocal other
+        if int(ids[0]) == at:   # another thread uploads while this chunk is read
+            other = threading.Thread(target=idx.upload_items, args=(np.zeros((10, 8), np.float32),))
+            other.start()
+            other.join(0.3)
+        return ids
+    idx.get_rows = get_rows
+    who = idx
+    if through_view:
+        who = engine.ItemIndex.__new__(engine.ItemIndex)
+        who.__dict__.update(idx.__dict__, _mu=threading.RLock(), _base=idx)
+    rows = who.quantize_items(chunk=4)
+    assert [r.tolist() for r in rows.got] == [[0, 1, 2, 3], [4, 5, 6, 7], [8, 9]]
+    other.join()
+    assert idx.quantized is None
+    who._mu = None   # (nothing to close)
