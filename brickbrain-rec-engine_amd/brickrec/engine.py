@@ -207,9 +207,10 @@ class ItemIndex:
                 n, d = rows.shape
                 rc = self._lib.bb_upload_items(self._h, rows.ctypes.data, n, d, _np_dtype_code(rows),
                                                int(prenormalized), L.BB_HOST, bp)
+            if rc not in (L.BB_E_ARG, L.BB_E_STATE):  # (refused before any row changed; any other failure leaves none to copy)
+                self._fp8 = None
             L.check(rc, "bb_upload_items")
             self.n_items, self.d = int(n), int(d)
-            self._fp8 = None
 
     def upload_cf(self, item_factors: np.ndarray, present: Optional[np.ndarray] = None):
         """CF item factors (n×r, same row space as the items) + presence mask (bool n)."""

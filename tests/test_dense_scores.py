@@ -90,3 +90,15 @@ def test_an_upload_waits_for_the_copy_and_drops_it(monkeypatch, at, through_view
     other.join()
     assert idx.quantized is None
     who._mu = None   # (nothing to close)
+
+
+@pytest.mark.parametrize("rc, kept", [(L.BB_E_ARG, True), (L.BB_E_STATE, True), (L.BB_E_HIP, False), (L.BB_E_NOMEM, False)])
+def test_a_failed_upload_drops_the_copy_and_a_refused_one_keeps_it(monkeypatch, rc, kept):
+    idx = _index(monkeypatch)
+    rows = idx.quantize_items()
+    assert idx.quantized is rows
+    idx._lib.rc = rc
+    monkeypatch.setattr(L, "load", lambda: idx._lib)
+    with pytest.raises(L.BrickrecError):
+        idx.upload_items(np.zeros((10, 8), np.float32))
+    assert (idx.quantized is rows) == kept
