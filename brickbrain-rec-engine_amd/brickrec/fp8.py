@@ -117,6 +117,8 @@ class Fp8Rows:
     def empty(cls, n: int, d: int, tile: bool = False, device=None) -> "Fp8Rows":
         """Rows to be written (``quantize_rows(..., out=...)``)."""
         dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise TypeError(f"rows are on a GPU: not on {dev}")
         kb = (d + 127) // 128
         sn = (n + 127) // 128 if tile else n
         new = cls.__new__(cls)
@@ -189,6 +191,8 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     rows may be strided, columns behind them stay as they were."""
     q, x = queries._codes, items._codes
     dev = q.get_device()
+    if dev < 0:
+        raise TypeError(f"rows are on a GPU: not on {q.device}")
     if x.get_device() != dev:
         raise ValueError("queries and items are on one device")
     if stream is not None:

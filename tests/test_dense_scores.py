@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from brickrec import _lib as L
-from brickrec import engine
+from brickrec import engine, fp8
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
@@ -102,3 +102,33 @@ def test_a_failed_upload_drops_the_copy_and_a_refused_one_keeps_it(monkeypatch, 
     with pytest.raises(L.BrickrecError):
         idx.upload_items(np.zeros((10, 8), np.float32))
     assert (idx.quantized is rows) == kept
+
+
+def _launches_nothing(monkeypatch):
+    """A library in which every launch is recorded instead: none may be reached with host memory."""
+    calls = []
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: calls.append(name) or 0
+    monkeypatch.setattr(L, "load", lambda: Lib())
+    monkeypatch.setattr(fp8, "_raw_stream", lambda dev: 0)
+    return calls
+
+
+@pytest.mark.parametrize("device", ["cpu", "meta"])
+def test_rows_are_made_on_a_gpu_only(monkeypatch, device):
+    calls = _launches_nothing(monkeypatch)
+    with pytest.raises(TypeError):
+        fp8.Fp8Rows.empty(3, 128, device=device)
+    # rows that came by other means: neither side may reach a launch
+    rows = fp8.Fp8Rows.__new__(fp8.Fp8Rows)
+    rows._codes = torch.empty((3, 128), dtype=torch.float8_e4m3fn, device=device)
+    rows._scales = torch.empty((1, 3), device=device)
+    rows._d, rows._tile = 128, False
+    rows._c = fp8._PACK(0, 0, 3, 128, 128, 3, False)
+    with pytest.raises(TypeError):
+        fp8.scores_fp8(rows, rows)
+    with pytest.raises(TypeError):
+        fp8.scores_fp8(rows, rows, out=torch.empty((3, 3), device=device))
+    assert calls == []
