@@ -29,6 +29,8 @@ from typing import Callable, Dict, List, Optional, Sequence
 
 import numpy as np
 
+from ._lib import BrickrecError
+
 RETRIEVER_K = 20   # lego_nlp_recommeder.py:305  search_kwargs={"k": 20}
 
 
@@ -125,7 +127,10 @@ class SemanticIndex:
 
     def scores(self, queries, **kw):
         """Dense scores [B, n] of query vectors against an 8-bit copy of the embeddings, with penalties,
-        biases and masks (``ItemIndex.scores``; the copy is made at the first call)."""
+        biases and masks (``ItemIndex.scores``; the copy is made at the first call).  Only an ``ItemIndex`` has
+        them: of a sharded index, each rank's ``local`` does."""
+        if not hasattr(self.index, "quantize_items"):
+            raise BrickrecError(f"dense scores need an ItemIndex: {type(self.index).__name__} has none")
         if self.index.quantized is None:
             self.index.quantize_items()
         q = np.asarray(queries, np.float32) if isinstance(queries, (list, tuple)) else queries

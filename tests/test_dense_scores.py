@@ -132,3 +132,11 @@ def test_rows_are_made_on_a_gpu_only(monkeypatch, device):
     with pytest.raises(TypeError):
         fp8.scores_fp8(rows, rows, out=torch.empty((3, 3), device=device))
     assert calls == []
+
+
+def test_semantic_scores_need_an_index_that_has_them():
+    from _oracle_index import OracleIndex
+    from brickrec.semantic import SemanticIndex
+    sem = SemanticIndex(["a", "b"], np.eye(2, 4), index_factory=OracleIndex)
+    with pytest.raises(L.BrickrecError, match="OracleIndex"):
+        sem.scores(np.ones(4))
