@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib as L
-from .fp8 import _CODE, _On, _check_out, _empty, _ld, _raw_stream, _refuse_grad, _rows_of
+from .fp8 import _CODE, _On, _check_out, _empty, _forward, _ld, _raw_stream, _refuse_grad, _rows_of
 
 Number = Union[float, torch.Tensor]
 
@@ -56,7 +56,7 @@ def _per_row(v: Number, name, B, dev):
         return 0, float(v), None
     if v.dtype is not _FLOAT or v.get_device() != dev or v.dim() != 1 or v.numel() != B:
         raise TypeError(f"{name} is a number or a float32 tensor [{B}] on cuda:{dev}")
-    if v.requires_grad:
+    if v.requires_grad or _forward._current_level >= 0:
         _refuse_grad(v)
     if not v.is_contiguous():
         v = v.contiguous()
@@ -88,7 +88,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         with _On(stream, scores.device, (scores, seen, seen_len, repetition, presence, frequency, bias_ids, bias, mask, out)):
             return adjust_scores(scores, seen=seen, seen_len=seen_len, repetition=repetition, presence=presence,
                                  frequency=frequency, bias_ids=bias_ids, bias=bias, mask=mask, out=out)
-    if scores.requires_grad:
+    if scores.requires_grad or _forward._current_level >= 0:
         _refuse_grad(scores)
     shape, dtype, dev = scores.shape, scores.dtype, scores.get_device()
     B, n = shape
@@ -129,7 +129,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         bias, m, ld_v = _list(bias, "bias", _F32, B, dev)
         if m != n_bias or bias.dim() != bias_ids.dim():
             raise ValueError(f"bias is as bias_ids: got {tuple(bias.shape)} and {tuple(bias_ids.shape)}")
-        if bias.requires_grad:
+        if bias.requires_grad or _forward._current_level >= 0:
             _refuse_grad(bias)
         if ld_v != ld_bias:  # (the two lists share one distance between rows)
             bias_ids, bias = bias_ids.contiguous(), bias.contiguous()

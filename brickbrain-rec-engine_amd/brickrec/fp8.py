@@ -5,7 +5,7 @@
 ``adjust.adjust_scores`` changes those before they are picked from.  A thin face of
 ``bb_quantize_fp8`` and ``bb_scores_fp8`` (include/brickrec.h), which say what is computed: torch CUDA
 tensors in and out, on torch's current stream or the ``stream`` given, no synchronisation, no state
-kept between calls.  No gradient flows through these calls, so inputs that ask for one are refused.
+kept between calls.  No gradient or tangent flows through these calls, so inputs that ask for one are refused.
 """
 from __future__ import annotations
 
@@ -14,6 +14,7 @@ import struct
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import _lib as L
 
@@ -29,8 +30,11 @@ def blocks_of(n: int) -> int:
 
 
 def _refuse_grad(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    """(Called where a tensor requires a gradient, or within a forward-mode level: _forward._current_level >= 0.)"""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError("no gradient flows through this call: detach the inputs or call it under torch.no_grad()")
+    if any(_forward.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError("no tangent flows through this call: unpack the inputs first")
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream, without the object (2 us a call)
@@ -108,7 +112,7 @@ class Fp8Rows:
             if n > 0 and kb > 0 and (codes.stride(1) != 1 or (sn > 1 and scales.stride(1) != 1)):
                 raise ValueError("codes and scales are contiguous along their rows")
             ld, sld = _ld(codes), _ld(scales)
-        if codes.requires_grad or scales.requires_grad:
+        if codes.requires_grad or scales.requires_grad or _forward._current_level >= 0:
             _refuse_grad(codes, scales)
         self._codes, self._scales, self._d, self._tile = codes, scales, d, bool(tile)
         self._c = _PACK(codes.data_ptr(), scales.data_ptr(), n, d, ld, sld, self._tile)
@@ -163,7 +167,7 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
         raise TypeError("rows are a float32, bfloat16 or float16 tensor on a GPU")
     if x.dim() != 2:
         raise ValueError(f"rows are [n, d]: got {tuple(x.shape)}")
-    if x.requires_grad:
+    if x.requires_grad or _forward._current_level >= 0:
         _refuse_grad(x)
     if stream is not None:
         with _On(stream, x.device, (x,) if out is None else (x, out.codes, out.scales)):
@@ -214,7 +218,7 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
 
 def _check_out(out, shape, dtype, dev):
     """The elements between the rows of a tensor to write into."""
-    if out.requires_grad:
+    if out.requires_grad or _forward._current_level >= 0:
         _refuse_grad(out)
     if out.dtype not in _CODE or (dtype is not None and out.dtype is not dtype):
         raise TypeError(f"out has dtype {out.dtype}")

@@ -528,3 +528,28 @@ def test_index_scores_of_any_magnitude(br):
     assert torch.equal(got[1], idx.scores(one[1:].to(DEV))[0])
     assert bool((got[3] == 0).all()) and bool(torch.isnan(got[4:]).all())
     idx.close()
+
+
+def test_tangents_are_refused(br):
+    from torch.autograd import forward_ad
+    q = quantized(br, 3, 200)
+    x, one = torch.randn((3, 200), device=DEV), torch.ones(3, device=DEV)
+    ids, bias = torch.zeros((3, 2), dtype=torch.int32, device=DEV), torch.ones((3, 2), device=DEV)
+    want = br.adjust_scores(x, seen=ids, repetition=one, presence=one, frequency=one, bias_ids=ids, bias=bias)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: br.quantize_rows(dual(x)), lambda: br.Fp8Rows(q.codes, dual(q.scales), 200),
+                     lambda: br.scores_fp8(q, q, out=dual(torch.empty((3, 3), device=DEV))),
+                     lambda: br.adjust_scores(dual(x)), lambda: br.adjust_scores(x, out=dual(torch.empty_like(x))),
+                     lambda: br.adjust_scores(x, seen=ids, repetition=dual(one)),
+                     lambda: br.adjust_scores(x, seen=ids, presence=dual(one)),
+                     lambda: br.adjust_scores(x, seen=ids, frequency=dual(one)),
+                     lambda: br.adjust_scores(x, bias_ids=ids, bias=dual(bias))):
+            with pytest.raises(ValueError):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError):     # (no_grad stops gradients, not tangents)
+                call()
+        got = br.adjust_scores(x, seen=ids, repetition=one, presence=one, frequency=one, bias_ids=ids, bias=bias)
+        assert torch.equal(got, want)                            # plain tensors within a level
+    with pytest.raises(ValueError):
+        torch.func.jvp(br.adjust_scores, (x,), (x,))
