@@ -179,6 +179,8 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
         out = Fp8Rows.empty(n, d, tile, x.device)
     elif (len(out), out._d, out._tile, out._codes.get_device()) != (n, d, bool(tile), dev):
         raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
+    elif out._scales.requires_grad:
+        _refuse_grad(out._scales)
     rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), out._c, _raw_stream(dev))
     if rc:
         L.check(rc, "bb_quantize_fp8")
@@ -199,6 +201,8 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
         raise TypeError(f"rows are on a GPU: not on {q.device}")
     if x.get_device() != dev:
         raise ValueError("queries and items are on one device")
+    if queries._scales.requires_grad or items._scales.requires_grad:  # (asked for after the rows were made)
+        _refuse_grad(queries._scales, items._scales)
     if stream is not None:
         with _On(stream, q.device, (q, queries.scales, x, items.scales, out)):
             return scores_fp8(queries, items, dtype=dtype, out=out)

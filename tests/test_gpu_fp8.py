@@ -553,3 +553,16 @@ def test_tangents_are_refused(br):
         assert torch.equal(got, want)                            # plain tensors within a level
     with pytest.raises(ValueError):
         torch.func.jvp(br.adjust_scores, (x,), (x,))
+
+
+def test_scales_that_come_to_ask_for_a_gradient(br):
+    q = quantized(br, 3, 200)
+    q.scales.requires_grad_()
+    with pytest.raises(ValueError):
+        br.scores_fp8(q, quantized(br, 4, 200))
+    with pytest.raises(ValueError):
+        br.scores_fp8(quantized(br, 4, 200), q)
+    with pytest.raises(ValueError):
+        br.quantize_rows(make(3, 200).to(DEV), out=q)
+    with torch.no_grad():
+        assert br.scores_fp8(q, q).shape == (3, 3)
