@@ -9,7 +9,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib as L
-from .fp8 import _CODE, _On, _check_out, _empty, _forward, _ld, _raw_stream, _refuse_grad, _rows_of
+from .fp8 import _CODE, _On, _check_out, _empty, _forward, _ld, _raw_stream, _refuse_grad, _rows_of, _wrote
 
 Number = Union[float, torch.Tensor]
 
@@ -96,7 +96,8 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     if not scores.is_contiguous():
         scores = _rows_of(scores)
         ld_scores = _ld(scores)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty(B, n, dtype, scores.device)
     else:
         ld = _check_out(out, shape, dtype, dev)
@@ -151,4 +152,6 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         _raw_stream(dev))
     if rc:
         L.check(rc, "bb_adjust_scores")
+    if given:
+        _wrote(out)
     return out

@@ -37,6 +37,13 @@ def _refuse_grad(*tensors):
         raise ValueError("no tangent flows through this call: unpack the inputs first")
 
 
+def _wrote(*outs):
+    """Tells autograd of a write into a caller's tensors, as torch's own calls do."""
+    for t in outs:
+        if not t.is_inference():  # (inference tensors have no version)
+            torch.autograd.graph.increment_version(t)
+
+
 _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream(device).cuda_stream, without the object (2 us a call)
 
 
@@ -174,8 +181,8 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
             return quantize_rows(x, tile=tile, out=out)
     x = _rows_of(x)
     n, d = x.shape
-    dev = x.get_device()
-    if out is None:
+    dev, given = x.get_device(), out is not None
+    if not given:
         out = Fp8Rows.empty(n, d, tile, x.device)
     elif (len(out), out._d, out._tile, out._codes.get_device()) != (n, d, bool(tile), dev):
         raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
@@ -184,6 +191,8 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
     rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), out._c, _raw_stream(dev))
     if rc:
         L.check(rc, "bb_quantize_fp8")
+    if given:
+        _wrote(out._codes, out._scales)
     return out
 
 
@@ -206,7 +215,8 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     if stream is not None:
         with _On(stream, q.device, (q, queries.scales, x, items.scales, out)):
             return scores_fp8(queries, items, dtype=dtype, out=out)
-    if out is None:
+    given = out is not None
+    if not given:
         if dtype not in _CODE:
             raise TypeError(f"scores are float32, bfloat16 or float16: not {dtype}")
         out = _empty(q.shape[0], x.shape[0], dtype, q.device)
@@ -217,6 +227,8 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
                                 _raw_stream(dev))
     if rc:
         L.check(rc, "bb_scores_fp8")
+    if given:
+        _wrote(out)
     return out
 
 

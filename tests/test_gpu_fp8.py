@@ -566,3 +566,38 @@ def test_scales_that_come_to_ask_for_a_gradient(br):
         br.quantize_rows(make(3, 200).to(DEV), out=q)
     with torch.no_grad():
         assert br.scores_fp8(q, q).shape == (3, 3)
+
+
+def test_writes_into_out_are_seen_by_autograd(br):
+    """A tensor that a backward pass has saved and that a call overwrites is torch's own error, not a wrong gradient."""
+    q = quantized(br, 4, 64)
+
+    def saved(shape):
+        y = torch.sigmoid(torch.randn(shape, device=DEV, requires_grad=True))   # (its backward reads y)
+        return y, y.detach()
+    y, out = saved((4, 4))
+    br.scores_fp8(q, q, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y, out = saved((4, 4))
+    br.adjust_scores(torch.zeros((4, 4), device=DEV), out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y, out = saved((4, 4))
+    br.adjust_scores(out, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y, out = saved((1, 4))
+    rows = br.Fp8Rows(q.codes, out, 64)
+    br.quantize_rows(make(2, 64).to(DEV), out=rows.part(1, 3))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    before = q.codes._version
+    br.quantize_rows(make(4, 64).to(DEV), out=q)
+    assert q.codes._version > before
+    with torch.inference_mode():                     # (such tensors have no version to advance)
+        o = torch.empty((4, 4), device=DEV)
+        want = br.scores_fp8(q, q)
+        assert torch.equal(br.scores_fp8(q, q, out=o), want)
+        assert torch.equal(br.adjust_scores(o, out=o), want)
+        assert br.quantize_rows(make(4, 64).to(DEV), out=br.Fp8Rows.empty(4, 64, device=DEV)).codes.shape == (4, 128)
