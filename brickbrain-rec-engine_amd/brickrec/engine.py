@@ -578,14 +578,16 @@ class ItemIndex:
         penalties, biases and mask of ``adjust.adjust_scores``, applied in place.  Every stored row gets
         a score; pass a mask to leave rows out.
 
-        Numpy in -> numpy out (f32); torch CUDA rows -> a torch tensor of ``dtype`` (f32 by default),
-        asynchronously on ``stream`` (default: torch's current stream)."""
+        Numpy in -> numpy out (f32); torch CUDA rows -> a torch tensor of ``dtype`` (that of ``out``, or f32, by
+        default), asynchronously on ``stream`` (default: torch's current stream)."""
         import torch
         from .adjust import adjust_scores
         from .fp8 import quantize_rows, scores_fp8
         items = self.quantized
         if items is None:
             raise L.BrickrecError("scores() needs quantize_items() first")
+        if out is not None and dtype not in (None, out.dtype):
+            raise TypeError(f"scores of {dtype} do not go into an out of {out.dtype}")
         dev = torch.device("cuda", self.device)
         host = not _is_torch(q_rows)
         if host:

@@ -140,3 +140,11 @@ def test_semantic_scores_need_an_index_that_has_them():
     sem = SemanticIndex(["a", "b"], np.eye(2, 4), index_factory=OracleIndex)
     with pytest.raises(L.BrickrecError, match="OracleIndex"):
         sem.scores(np.ones(4))
+
+
+def test_dtype_and_out_agree(monkeypatch):
+    idx = _index(monkeypatch)
+    idx.quantize_items()
+    for q in (np.zeros((2, 8), np.float32), types.SimpleNamespace()):
+        with pytest.raises(TypeError, match="out"):
+            idx.scores(q, dtype=torch.float32, out=torch.empty((2, 10), dtype=torch.bfloat16))
