@@ -578,7 +578,7 @@ class ItemIndex:
         penalties, biases and mask of ``adjust.adjust_scores``, applied in place.  Every stored row gets
         a score; pass a mask to leave rows out.
 
-        Numpy in -> numpy out (f32); torch CUDA rows -> a torch tensor of ``dtype`` (that of ``out``, or f32, by
+        Numpy in -> numpy out (f32), and the adjustment's lists and mask may be numpy arrays too; torch CUDA rows -> a torch tensor of ``dtype`` (that of ``out``, or f32, by
         default), asynchronously on ``stream`` (default: torch's current stream)."""
         import torch
         from .adjust import adjust_scores
@@ -609,6 +609,8 @@ class ItemIndex:
         with torch.cuda.stream(s):
             if host:
                 q_rows = torch.from_numpy(q_rows).to(dev)
+                adjust = {k: torch.from_numpy(np.ascontiguousarray(v)).to(dev) if isinstance(v, np.ndarray) else v
+                          for k, v in adjust.items()}
             q = q_rows
             if normalize:
                 q = _unit_rows(q if q.dtype in (torch.float32, torch.float64) else q.float())

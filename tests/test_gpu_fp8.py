@@ -601,3 +601,24 @@ def test_writes_into_out_are_seen_by_autograd(br):
         assert torch.equal(br.scores_fp8(q, q, out=o), want)
         assert torch.equal(br.adjust_scores(o, out=o), want)
         assert br.quantize_rows(make(4, 64).to(DEV), out=br.Fp8Rows.empty(4, 64, device=DEV)).codes.shape == (4, 128)
+
+
+def test_index_scores_with_numpy_lists(br):
+    n, d, B = 1000, 64, 3
+    idx = br.ItemIndex()
+    idx.upload_items(make(n, d, seed=1).numpy())
+    idx.quantize_items()
+    q = make(B, d, seed=2).numpy()
+    kw = {"seen": np.array([[5, 7, 7, -1]] * B, np.int32), "seen_len": np.array([4, 3, 0], np.int32), "repetition": np.full(B, 1.5, np.float32),
+          "presence": 0.25, "frequency": 0.5, "bias_ids": np.array([3, 9], np.int32), "bias": np.array([1.0, -2.0], np.float32)}
+    allowed = np.random.default_rng(1).random((B, n)) < 0.5
+    dev = {k: torch.from_numpy(v).to(DEV) if isinstance(v, np.ndarray) else v for k, v in kw.items()}
+    want = idx.scores(torch.from_numpy(q).to(DEV), mask=torch.from_numpy(allowed).to(DEV), **dev).cpu().numpy()
+    for mask in (allowed, br.bits_from_bool(allowed)):
+        assert np.array_equal(idx.scores(q, mask=mask, **kw), want)
+    assert np.array_equal(idx.scores(q, mask=torch.from_numpy(allowed).to(DEV), **{**kw, "seen": dev["seen"]}), want)
+    with pytest.raises(TypeError):
+        idx.scores(q, bias_ids=kw["bias_ids"], bias=kw["bias"].astype(np.float64))
+    with pytest.raises(TypeError):
+        idx.scores(torch.from_numpy(q).to(DEV), seen=kw["seen"])    # torch rows take torch lists
+    idx.close()
