@@ -107,13 +107,13 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     rep, pre, fre = 1.0, 0.0, 0.0
     if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
         raise ValueError(f"repetition is above 0: got {repetition}")
-    if seen is not None and bias_ids is not None and seen.dtype is not bias_ids.dtype and {seen.dtype, bias_ids.dtype} == _IDS.keys():
+    if isinstance(seen, torch.Tensor) and isinstance(bias_ids, torch.Tensor) and seen.dtype is not bias_ids.dtype and {seen.dtype, bias_ids.dtype} == _IDS.keys():
         seen, bias_ids = seen.to(torch.int64), bias_ids.to(torch.int64)  # (the lists of one call have ids of one size)
     if seen is not None:
         seen, n_seen, ld_seen = _list(seen, "seen", _IDS, B, dev)
         seen_p, ids64 = seen.data_ptr(), int(seen.dtype is torch.int64)
         if seen_len is not None:
-            if seen_len.dtype is not torch.int32 or seen_len.get_device() != dev or seen_len.dim() != 1 or seen_len.numel() != B:
+            if not isinstance(seen_len, torch.Tensor) or seen_len.dtype is not torch.int32 or seen_len.get_device() != dev or seen_len.dim() != 1 or seen_len.numel() != B:
                 raise TypeError(f"seen_len is an int32 tensor [{B}] on cuda:{dev}")
             if not seen_len.is_contiguous():
                 seen_len = seen_len.contiguous()
@@ -138,7 +138,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
         bias_ids_p, bias_p = bias_ids.data_ptr(), bias.data_ptr()
         ids64 = int(bias_ids.dtype is torch.int64)
     if mask is not None:
-        if mask.dtype is _BOOL:
+        if isinstance(mask, torch.Tensor) and mask.dtype is _BOOL:
             if mask.dim() == 0 or mask.shape[-1] != n:
                 raise ValueError(f"a bool mask is [{n}] or [{B}, {n}]: got {tuple(mask.shape)}")
             mask = mask_words(mask)

@@ -102,6 +102,8 @@ class Fp8Rows:
     tile = property(operator.attrgetter("_tile"), doc="whether a scale covers 128 rows")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, d: int, tile: bool = False):
+        if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+            raise TypeError("codes and scales are tensors")
         if codes.dtype is not _E4M3 or scales.dtype is not _F32:
             raise TypeError(f"codes are float8_e4m3fn and scales float32: got {codes.dtype} and {scales.dtype}")
         if not codes.is_cuda or scales.get_device() != codes.get_device():
@@ -172,6 +174,8 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
     write into."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype not in _CODE:
         raise TypeError("rows are a float32, bfloat16 or float16 tensor on a GPU")
+    if out is not None and not isinstance(out, Fp8Rows):
+        raise TypeError(f"out is Fp8Rows: got {type(out).__name__}")
     if x.dim() != 2:
         raise ValueError(f"rows are [n, d]: got {tuple(x.shape)}")
     if x.requires_grad or _forward._current_level >= 0:
@@ -204,6 +208,8 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     the sum of the products' magnitudes in all; f32 and f16 scores lose nothing there.  The queries' scales are per
     row; the items' per row or per tile.  ``out``: a tensor of that shape (its dtype is then the scores') to write into; its
     rows may be strided, columns behind them stay as they were."""
+    if not isinstance(queries, Fp8Rows) or not isinstance(items, Fp8Rows):
+        raise TypeError(f"queries and items are Fp8Rows: got {type(queries).__name__} and {type(items).__name__}")
     q, x = queries._codes, items._codes
     dev = q.get_device()
     if dev < 0:
@@ -234,6 +240,8 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
 
 def _check_out(out, shape, dtype, dev):
     """The elements between the rows of a tensor to write into."""
+    if not isinstance(out, torch.Tensor):
+        raise TypeError(f"out is a tensor: got {type(out).__name__}")
     if out.requires_grad or _forward._current_level >= 0:
         _refuse_grad(out)
     if out.dtype not in _CODE or (dtype is not None and out.dtype is not dtype):

@@ -274,3 +274,14 @@ def test_replayed_with_a_bool_mask(br, B, n):
         torch.cuda.synchronize()
         assert torch.equal(out, scores.masked_fill(~mask, -INF)), s
         out.clamp(min=0).sum().item()
+
+
+def test_what_is_no_tensor_is_a_type_error(br):
+    s = torch.zeros((2, 64), device=DEV)
+    ids = torch.zeros((2, 3), dtype=torch.int32, device=DEV)
+    one = torch.ones((2, 3), device=DEV)
+    for kw in ({"seen": [1, 2]}, {"seen": [[1], [2]], "bias_ids": ids, "bias": one}, {"seen": ids, "bias_ids": [1, 2, 3], "bias": one},
+               {"seen": ids, "seen_len": [3, 3]}, {"bias_ids": ids, "bias": [1.0, 2.0, 3.0]}, {"mask": [True] * 64},
+               {"mask": bytes(8)}, {"seen": ids, "repetition": [1.0, 2.0]}, {"seen": ids, "presence": "much"}, {"out": [0.0]}):
+        with pytest.raises((TypeError, ValueError)):
+            br.adjust_scores(s, **kw)

@@ -622,3 +622,12 @@ def test_index_scores_with_numpy_lists(br):
     with pytest.raises(TypeError):
         idx.scores(torch.from_numpy(q).to(DEV), seen=kw["seen"])    # torch rows take torch lists
     idx.close()
+
+
+def test_what_are_no_rows_is_a_type_error(br):
+    q = quantized(br, 3, 200)
+    for call in (lambda: br.scores_fp8(q.codes, q), lambda: br.scores_fp8(q, None), lambda: br.scores_fp8(q, q, out=[0.0]),
+                 lambda: br.quantize_rows(make(3, 200).to(DEV), out=q.codes), lambda: br.quantize_rows([[1.0]]),
+                 lambda: br.Fp8Rows([1], q.scales, 200), lambda: br.Fp8Rows(q.codes, None, 200)):
+        with pytest.raises(TypeError):
+            call()
