@@ -18,9 +18,10 @@ def mask_words(mask: torch.Tensor) -> torch.Tensor:
     """bool [..., n] on a GPU -> int32 words [..., ⌈n/32⌉], bit i of word w = entry 32w + i: the layout of
     ``ItemIndex.eval_mask_bits`` and ``engine.bits_from_bool``, packed on the device."""
     n = mask.shape[-1]
-    pad = torch.nn.functional.pad(mask, (0, -n % 32)).view(*mask.shape[:-1], (n + 31) // 32, 32)
-    bit = torch.arange(32, device=mask.device)
-    return (pad.to(torch.int64) << bit).sum(-1).to(torch.int32)
+    pad = torch.nn.functional.pad(mask, (0, -n % 32)).contiguous().view(torch.uint8)
+    bit = torch.arange(8, dtype=torch.uint8, device=mask.device)
+    # (8 bits to a byte, 4 bytes to a word: two bytes a score besides the words)
+    return (pad.view(*mask.shape[:-1], (n + 31) // 32, 4, 8) << bit).sum(-1, dtype=torch.uint8).view(torch.int32).squeeze(-1)
 
 
 # bb_adjust packed into bytes (a third of the time of a ctypes structure); its fields in order
@@ -79,7 +80,7 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     seen, bias_ids: int32 or int64, [B, m] or [m] for all rows; ids outside [0, n) are skipped (pad with
     -1).  seen_len: int32 [B].  repetition (> 0), presence, frequency: numbers, or f32 [B].  bias: f32, as
     bias_ids.  mask: words [⌈n/32⌉] or [B, ⌈n/32⌉] (``ItemIndex.eval_mask_bits``), or bool [n] or [B, n],
-    which costs a few launches more.  out: where to write; may be ``scores`` itself."""
+    which costs a few launches and two bytes of memory a score more.  out: where to write; may be ``scores`` itself."""
     if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _CODE:
         raise TypeError("scores are a float32, bfloat16 or float16 tensor on a GPU")
     if scores.dim() != 2:

@@ -285,3 +285,26 @@ def test_what_is_no_tensor_is_a_type_error(br):
                {"mask": bytes(8)}, {"seen": ids, "repetition": [1.0, 2.0]}, {"seen": ids, "presence": "much"}, {"out": [0.0]}):
         with pytest.raises((TypeError, ValueError)):
             br.adjust_scores(s, **kw)
+
+
+def test_mask_words_take_little_memory(br):
+    """One byte a score for the padded copy, one for its shifted bits, an eighth for the words, and room for the allocator's
+    rounding of each."""
+    m = torch.ones((64, 131001), dtype=torch.bool, device=DEV)
+    br.mask_words(m)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    w = br.mask_words(m)
+    assert torch.cuda.max_memory_allocated() - before <= 2.25 * m.numel() + (1 << 20)
+    assert w.shape == (64, 4094) and w.dtype == torch.int32
+    assert bool((w[:, :-1] == -1).all()) and bool((w[:, -1] == (1 << 131001 % 32) - 1).all())
+
+
+@pytest.mark.parametrize("shape", [(1,), (31,), (32,), (33,), (2, 3, 70), (0, 5), (4, 0)])
+def test_mask_words_of_any_shape(br, shape):
+    from brickrec.engine import bits_from_bool
+    import numpy as np
+    m = torch.rand(shape, generator=torch.Generator().manual_seed(2)) < 0.5
+    for t in (m.to(DEV), torch.stack((m, m), -1).to(DEV)[..., 0]):      # (and one whose scores lie apart)
+        assert np.array_equal(br.mask_words(t).cpu().numpy().view(np.uint32), bits_from_bool(m.numpy()))
