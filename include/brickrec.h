@@ -307,8 +307,9 @@ int bb_quantize_fp8(int32_t device, const void* x, int32_t dtype, int64_t ldx, c
 /* out[m][n] = <q row m, item row n> for every pair, ldo elements between rows of out, dtype BB_F32 /
  * BB_BF16 / BB_F16 (rounded once, to nearest even).  q->d == items->d; q->tile must be 0.
  * Products of codes are summed in f32 over each block of 128, then multiplied by the two
- * scales (their product first) and summed over the blocks in f32, in ascending order up to a split
- * into a few parts; the order depends on the sizes alone, so equal calls give equal bits.
+ * scales (their product first: where it leaves f32's range the block counts as 0, an infinity or, if its products sum
+ * to 0, NaN) and summed over the blocks in f32, in ascending order up to a split into a few parts.  The order
+ * depends on the sizes, the type and whether rows lie 2^24 bytes or more apart, so equal calls give equal bits.
  * For BB_F32 and BB_F16 the products enter these sums whole.  For BB_BF16 they come from the 8-bit matrix
  * instruction, at up to twice the rate: it cuts each product at 2^-13 of the largest of its group of 8
  * columns, which takes at most 2^-10 of the sum of magnitudes sum_k |q_k x_k| from a score (bf16 rounds by
