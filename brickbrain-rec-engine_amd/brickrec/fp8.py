@@ -95,7 +95,7 @@ class Fp8Rows:
     codes[i, j] · scales[j // 128, i or i // 128].  The calls use the tensors' memory as it is when the
     rows are made: their contents may change after that, their storage may not be resized or replaced."""
 
-    __slots__ = ("_codes", "_scales", "_d", "_tile", "_c")
+    __slots__ = ("_codes", "_scales", "_d", "_tile", "_c", "_cut")  # (_cut: other rows share the last tile's scale)
     codes = property(operator.attrgetter("_codes"), doc="float8_e4m3fn [n, 128·⌈d/128⌉]")
     scales = property(operator.attrgetter("_scales"), doc="f32 [⌈d/128⌉, n], or [⌈d/128⌉, ⌈n/128⌉] with tile")
     d = property(operator.attrgetter("_d"), doc="columns of a row")
@@ -123,7 +123,7 @@ class Fp8Rows:
             ld, sld = _ld(codes), _ld(scales)
         if codes.requires_grad or scales.requires_grad or _forward._current_level >= 0:
             _refuse_grad(codes, scales)
-        self._codes, self._scales, self._d, self._tile = codes, scales, d, bool(tile)
+        self._codes, self._scales, self._d, self._tile, self._cut = codes, scales, d, bool(tile), False
         self._c = _PACK(codes.data_ptr(), scales.data_ptr(), n, d, ld, sld, self._tile)
 
     @classmethod
@@ -137,7 +137,7 @@ class Fp8Rows:
         new = cls.__new__(cls)
         new._codes = _empty(n, kb * BLOCK, _E4M3, dev)
         new._scales = _empty(kb, sn, _F32, dev)
-        new._d, new._tile = d, bool(tile)
+        new._d, new._tile, new._cut = d, bool(tile), False
         new._c = _PACK(new._codes.data_ptr(), new._scales.data_ptr(), n, d, kb * BLOCK or 1, sn or 1, new._tile)
         return new
 
@@ -152,11 +152,14 @@ class Fp8Rows:
         return self.codes.device
 
     def part(self, start: int, stop: int) -> "Fp8Rows":
-        """Rows [start, stop) as a view; with ``tile`` a start that is a multiple of 128."""
+        """Rows [start, stop) as a view; with ``tile`` a start that is a multiple of 128, and a view that ends inside
+        a tile is for reading."""
         if not 0 <= start <= stop <= len(self) or (self.tile and start % BLOCK):
             raise ValueError(f"no part [{start}, {stop}) of {len(self)} rows")
         a, b = (start // BLOCK, blocks_of(stop)) if self.tile else (start, stop)
-        return Fp8Rows(self.codes[start:stop], self.scales[:, a:b], self.d, self.tile)
+        new = Fp8Rows(self.codes[start:stop], self.scales[:, a:b], self.d, self.tile)
+        new._cut = self.tile and stop % BLOCK > 0 and (stop < len(self) or self._cut)
+        return new
 
     def dequantize(self) -> torch.Tensor:
         """The rows as f32 [n, d] (for inspection: the scores are computed from the codes)."""
@@ -190,6 +193,8 @@ def quantize_rows(x: torch.Tensor, *, tile: bool = False, out: Optional[Fp8Rows]
         out = Fp8Rows.empty(n, d, tile, x.device)
     elif (len(out), out._d, out._tile, out._codes.get_device()) != (n, d, bool(tile), dev):
         raise ValueError(f"out is {len(out)} rows {out.d} wide (tile={out.tile}) on {out.device}, not as x and tile ask")
+    elif out._cut:
+        raise ValueError(f"out ends inside a tile of 128 rows, whose scale the rows behind it share: {len(out)} rows")
     elif out._scales.requires_grad:
         _refuse_grad(out._scales)
     rc = L.load().bb_quantize_fp8(dev, x.data_ptr(), _CODE[x.dtype], _ld(x), out._c, _raw_stream(dev))

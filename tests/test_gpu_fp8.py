@@ -631,3 +631,20 @@ def test_what_are_no_rows_is_a_type_error(br):
                  lambda: br.Fp8Rows([1], q.scales, 200), lambda: br.Fp8Rows(q.codes, None, 200)):
         with pytest.raises(TypeError):
             call()
+
+
+def test_no_quantizing_into_part_of_a_tile(br):
+    """A tile has one scale: writing some of its rows would change the values of the others."""
+    x = make(300, 200, seed=1).to(DEV)
+    rows = br.quantize_rows(x, tile=True)
+    want = rows.dequantize()
+    for part in (rows.part(0, 100), rows.part(128, 299), rows.part(0, 256).part(128, 130), rows.part(0, 140).part(128, 140)):
+        with pytest.raises(ValueError):
+            br.quantize_rows(100 * x[:len(part)], tile=True, out=part)
+    assert torch.equal(rows.dequantize(), want)
+    assert torch.equal(rows.part(0, 100).dequantize(), want[:100])      # reading is another matter
+    for a, b in ((0, 128), (128, 256), (256, 300), (128, 300), (0, 300)):
+        br.quantize_rows(x[a:b], tile=True, out=rows.part(a, b))
+    assert torch.equal(rows.dequantize(), want)
+    plain = br.quantize_rows(x)
+    br.quantize_rows(x[5:9], out=plain.part(5, 9))                      # a row has its own scales
