@@ -64,10 +64,11 @@ def _unit_rows(q):
     import torch
     word, exponent, least = {torch.float32: (torch.int32, 0x7F800000, 2.0 ** -126),
                              torch.float64: (torch.int64, 0x7FF0000000000000, 2.0 ** -1022)}[q.dtype]
-    top = torch.linalg.vector_norm(q, float("inf"), dim=1, keepdim=True)
-    power = (top.view(word) & exponent).view(q.dtype).clamp_min_(least)
+    power = torch.linalg.vector_norm(q, float("inf"), 1, True)
+    power.view(word).bitwise_and_(exponent)
+    q = q / power.clamp_min_(least)
     # (the norm of a row that is not zero is now at least 1, or 2^-23 (2^-52) for the smallest numbers)
-    return torch.nn.functional.normalize(q / power, dim=1, eps=1e-30)
+    return q.div_(torch.linalg.vector_norm(q, 2, 1, True).clamp_min_(1e-30))
 
 
 def _torch_dtype_code(t) -> int:
