@@ -210,7 +210,7 @@ using Mode = std::conditional_t<std::is_same_v<T, __bf16>, Narrow, Wide>;
 // ---- the product of few rows -----------------------------------------------------------------
 // Bound by reading the items once: operands go straight from memory to registers, up to PF blocks
 // of a wave in flight.  A workgroup takes 16 items x 16 queries; its KS waves take every KS-th block of the
-// same rows and are summed through LDS, in order of the wave.  1 x 25,216 x 384 to f32: 4.1 us, of which the launch
+// same rows and are summed through LDS, in order of the wave.  1 x 25,216 x 384 to f32: 3.9 us, of which the launch
 // is 2; 1 x 100,000 x 768: 15.5 us, 5.0 TB/s.
 template <typename T, int KS, int PF>
 __global__ __launch_bounds__(KS * 64) void product_few_kernel(ProductArgs a, int n_groups) {
@@ -543,10 +543,11 @@ __global__ __launch_bounds__(KG* WN* WM * 64, KG* WN* WM > 8 ? KG * WN * WM / 4 
 //  - a product is scaled three products later.  The empty asm keeps the compiler from collecting the sums at the
 //    end of the block, which would hold all 32 products in registers.
 // 4,096 x 8,192 x 4,096: 118 us, 2.33 PFLOP/s (135 us with a workgroup to a tile; 3.2 PFLOP/s is what a large 8-bit
-// product without block scales reaches).  4,096 x 125,000 x 768, whose rows begin anywhere in a line: 625 us against
-// 743 with tiles of 128 and 722 with 128 bytes of a row to a store; with 124,992 items, whose rows begin at
-// lines, 128 bytes take 545 us and 512 take 615.  The clock falls to 1.8 to 1.9 GHz under
-// this load (2.4 without): the same product of rows that are all alike, whose wires hardly switch, is 11 to 13 % faster.
+// product without block scales reaches).  4,096 x 125,000 x 768, whose rows begin anywhere in a line, measured in turn: 625 us
+// against 743 with tiles of 128 and 722 with 128 bytes of a row to a store; with 124,992 items, whose rows begin at
+// lines, 128 bytes take 545 us and 512 take 615.  (506 us over the same tensors again and again, 655 over inputs that change.)
+// The clock falls to 2.0 to 2.1 GHz under this load (2.4 without): the same product of rows that are all alike, whose
+// wires hardly switch, is 12 to 16 % faster.
 template <typename T>
 using RunShape = TileShape<T, 4, 2, 8, 2, 1>;  // 256 x 256
 constexpr int kCus = 256;
