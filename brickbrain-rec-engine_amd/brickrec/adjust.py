@@ -18,7 +18,7 @@ def mask_words(mask: torch.Tensor) -> torch.Tensor:
     """bool [..., n] on a GPU -> int32 words [..., ⌈n/32⌉], bit i of word w = entry 32w + i: the layout of
     ``ItemIndex.eval_mask_bits`` and ``engine.bits_from_bool``, packed on the device."""
     n = mask.shape[-1]
-    pad = torch.nn.functional.pad(mask, (0, -n % 32)).contiguous().view(torch.uint8)
+    pad = torch.nn.functional.pad(mask.bool(), (0, -n % 32)).contiguous().view(torch.uint8)
     bit = torch.arange(8, dtype=torch.uint8, device=mask.device)
     # (8 bits to a byte, 4 bytes to a word: two bytes a score besides the words)
     return (pad.view(*mask.shape[:-1], (n + 31) // 32, 4, 8) << bit).sum(-1, dtype=torch.uint8).view(torch.int32).squeeze(-1)
@@ -108,13 +108,14 @@ def adjust_scores(scores: torch.Tensor, *, seen: Optional[torch.Tensor] = None,
     rep, pre, fre = 1.0, 0.0, 0.0
     if not isinstance(repetition, torch.Tensor) and not repetition > 0.0:
         raise ValueError(f"repetition is above 0: got {repetition}")
-    if isinstance(seen, torch.Tensor) and isinstance(bias_ids, torch.Tensor) and seen.dtype is not bias_ids.dtype and {seen.dtype, bias_ids.dtype} == _IDS.keys():
+    if isinstance(seen, torch.Tensor) and isinstance(bias_ids, torch.Tensor) and {seen.dtype, bias_ids.dtype} == _IDS.keys():
         seen, bias_ids = seen.to(torch.int64), bias_ids.to(torch.int64)  # (the lists of one call have ids of one size)
     if seen is not None:
         seen, n_seen, ld_seen = _list(seen, "seen", _IDS, B, dev)
         seen_p, ids64 = seen.data_ptr(), int(seen.dtype is torch.int64)
         if seen_len is not None:
-            if not isinstance(seen_len, torch.Tensor) or seen_len.dtype is not torch.int32 or seen_len.get_device() != dev or seen_len.dim() != 1 or seen_len.numel() != B:
+            if (not isinstance(seen_len, torch.Tensor) or seen_len.dtype is not torch.int32 or seen_len.get_device() != dev
+                    or seen_len.dim() != 1 or seen_len.numel() != B):
                 raise TypeError(f"seen_len is an int32 tensor [{B}] on cuda:{dev}")
             if not seen_len.is_contiguous():
                 seen_len = seen_len.contiguous()

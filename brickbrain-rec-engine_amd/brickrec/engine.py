@@ -573,14 +573,14 @@ class ItemIndex:
     def scores(self, q_rows, *, normalize: bool = True, dtype=None, stream=None, out=None, **adjust):
         """Dense scores [B, n] of query rows against the 8-bit copy of the items (``quantize_items``,
         called first): column j is item id_offset + j.  The queries are L2-normalised unless
-        ``normalize`` is False (in their own type, f64 rows in f64, others in f32; a zero row scores 0), then quantised
-        as the items are; the scores
-        are those of the 8-bit rows, not the exact ones that ``search`` ranks by.  ``adjust``: the
-        penalties, biases and mask of ``adjust.adjust_scores``, applied in place.  Every stored row gets
-        a score; pass a mask to leave rows out.
+        ``normalize`` is False (f64 rows in f64, others in f32; a zero row scores 0), then quantised as
+        the items are; the scores are those of the 8-bit rows, not the exact ones that ``search`` ranks
+        by.  ``adjust``: the penalties, biases and mask of ``adjust.adjust_scores``, applied in place.
+        Every stored row gets a score; pass a mask to leave rows out.
 
-        Numpy in -> numpy out (f32), and the adjustment's lists and mask may be numpy arrays too; torch CUDA rows -> a torch tensor of ``dtype`` (that of ``out``, or f32, by
-        default), asynchronously on ``stream`` (default: torch's current stream)."""
+        Numpy in -> numpy out (f32), and the adjustment's lists and mask may be numpy arrays too; torch
+        CUDA rows -> a torch tensor of ``dtype`` (that of ``out``, or f32, by default), asynchronously on
+        ``stream`` (default: torch's current stream)."""
         import torch
         from .adjust import adjust_scores
         from .fp8 import quantize_rows, scores_fp8

@@ -210,9 +210,9 @@ def scores_fp8(queries: Fp8Rows, items: Fp8Rows, *, dtype: torch.dtype = torch.f
     """Dense scores [queries, items] of 8-bit rows: the inner product of every pair, accumulated in f32 and
     rounded once to ``dtype`` (f32, bf16 or f16).  bf16 scores come from the 8-bit matrix instruction, at up to
     twice the rate: it cuts each product at 2^-13 of the largest of its group of 8 columns, at most 2^-10 of
-    the sum of the products' magnitudes in all; f32 and f16 scores lose nothing there.  The queries' scales are per
-    row; the items' per row or per tile.  ``out``: a tensor of that shape (its dtype is then the scores') to write into; its
-    rows may be strided, columns behind them stay as they were."""
+    the sum of the products' magnitudes in all; f32 and f16 scores lose nothing there.  The queries' scales are
+    per row; the items' per row or per tile.  ``out``: a tensor of that shape (its dtype is then the scores') to
+    write into; its rows may be strided, columns behind them stay as they were."""
     if not isinstance(queries, Fp8Rows) or not isinstance(items, Fp8Rows):
         raise TypeError(f"queries and items are Fp8Rows: got {type(queries).__name__} and {type(items).__name__}")
     q, x = queries._codes, items._codes

@@ -148,3 +148,10 @@ def test_dtype_and_out_agree(monkeypatch):
     for q in (np.zeros((2, 8), np.float32), types.SimpleNamespace()):
         with pytest.raises(TypeError, match="out"):
             idx.scores(q, dtype=torch.float32, out=torch.empty((2, 10), dtype=torch.bfloat16))
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.uint8, torch.int32, torch.float32])
+def test_mask_words_of_any_type(dtype):
+    from brickrec.adjust import mask_words
+    m = torch.rand((2, 70), generator=torch.Generator().manual_seed(1)) < 0.5
+    assert np.array_equal(mask_words(m.to(dtype)).numpy().view(np.uint32), engine.bits_from_bool(m.numpy()))
